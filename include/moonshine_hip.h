@@ -316,6 +316,104 @@ MSH_EXPORT int64_t msh_host_biaser_bonuses(const int32_t* flat_tokens, const int
                                            uint64_t vocab);
 
 /* ---------------------------------------------------------------------------------------------------
+ * Serving operators on device memory: a paged key / value cache held in 4 bits with the attention that reads it, and the two
+ * steps of a beam search.  (No reference counterpart: its decoder keeps fp32 caches, core/moonshine-model.cpp:354-368, and
+ * decodes greedily, :454-470.)  The engine calls them for kv_dtype = 2 and for beam widths above 1; a host with a decoder of its
+ * own calls them here.
+ *
+ * All pointers are device pointers of `device`; `stream` is a hipStream_t of that device (NULL: its default stream).  The calling
+ * thread's current device is left as it was.  Calls enqueue and return: nothing is allocated, copied or waited for, no state is kept
+ * between calls, so any number of threads and streams may call at once and every call may be captured into a graph -- with a
+ * workspace of its own for each call that can run at the same time.  Results do not depend on what else runs (no atomics).
+ * Return 0 or a negative msh_status; msh_op_last_error() is the calling thread's message.
+ * ------------------------------------------------------------------------------------------------- */
+enum msh_dtype { MSH_F32 = 0, MSH_BF16 = 1, MSH_F16 = 2 };
+
+MSH_EXPORT const char* msh_op_last_error(void);
+
+/* A cache: `pages` pages of page_size tokens (a power of two >= 32) for `heads` key / value heads of head_dim <= 256 elements, at
+ * `data` (16-byte aligned, pages * msh_kv4_page_bytes() bytes).  Token t of a page is slot page * page_size + t.  Every 32 elements of
+ * a token's key or value share a power of two, each is one of 0, +-.5, 1, 1.5, 2, 3, 4, 6 times it (OCP MX fp4: 4.25 bits an element;
+ * the power is floor(log2(amax)) - 2, one more where amax is 1.75 times a power of two or above).  The byte layout is the attention
+ * kernel's (csrc/serve_kernels.h) and private to these calls. */
+typedef struct msh_kv4_cache {
+  void* data;
+  int64_t pages;
+  int32_t heads, page_size, head_dim;
+} msh_kv4_cache;
+MSH_EXPORT int64_t msh_kv4_page_bytes(int32_t heads, int32_t page_size, int32_t head_dim);
+
+/* Block table and slot map of a step, from the requests' lengths.  Request b holds kv_lens[b] tokens after the step, the last
+ * new_lens[b] of them in rows row_start[b], row_start[b] + 1, ... of the step's packed rows.  Row b of block_table [batch][table_width]
+ * keeps its entries for the tokens held before, gets pages from free_pages (in order: request by request) for the others, and -1 behind
+ * them.  slots [rows] receives every row's slot, -1 for rows of no request.  used[0] = pages taken from free_pages; if it exceeds
+ * n_free, the entries that found no page and the slots in them are -1.  Lengths are cut to [0, table_width * page_size], new_lens to
+ * [0, kv_lens].  The rows of two requests must not overlap and row_start must not decrease. */
+MSH_EXPORT int32_t msh_page_plan(int32_t device, void* stream, int32_t* block_table, int32_t batch, int32_t table_width,
+                                 const int32_t* kv_lens, const int32_t* new_lens, const int32_t* row_start, int64_t rows,
+                                 const int32_t* free_pages, int64_t n_free, int32_t page_size, int64_t* slots, int32_t* used);
+
+/* Write `rows` keys and values [rows][heads][head_dim] (element strides: row, head, element) into their slots; a slot that is negative
+ * or past the cache is skipped.  The slots of a call must differ (else the token is one of the rows' or a mix of them).  NaN is
+ * stored as 0, infinities as the largest finite value; a group below 2^-102 becomes 0.
+ * msh_kv4_read: the values of slots, contiguous [rows][heads][head_dim]; zeros for a slot that is not in the cache. */
+MSH_EXPORT int32_t msh_kv4_write(int32_t device, void* stream, const msh_kv4_cache* cache, const void* k, const int64_t* k_strides,
+                                 const void* v, const int64_t* v_strides, int32_t dtype, int64_t rows, const int64_t* slots);
+MSH_EXPORT int32_t msh_kv4_read(int32_t device, void* stream, const msh_kv4_cache* cache, const int64_t* slots, int64_t rows, void* k,
+                                void* v, int32_t dtype);
+
+/* out[r, h] = softmax(scale * q[r, h] . K) V over the cached tokens of row r's sequence; query head h reads cache head
+ * h / (heads / cache.heads).  Sequence b has rows q_start[b] .. q_start[b + 1] - 1 (at most max_q of them; NULL: max_q rows each) and
+ * kv_lens[b] tokens in the pages block_table[b][..].  causal: the rows are its LAST tokens, row i sees the tokens up to and including
+ * kv_lens[b] - n_rows + i, of these only the last `window` if window > 0; otherwise every row sees all.  A row that sees nothing gets
+ * zeros and lse = -inf.  Tokens in a page that is not in the cache count as masked.  Rows of no sequence are left as they are; lse
+ * [rows][heads] (nullable) is the natural logarithm of the sum of exponentials.  out has q's type.  Sums and the softmax are fp32;
+ * bf16 outputs take p as two bf16 terms, fp32 ones as three.  The number of key ranges, and so the summation order, goes by the sizes
+ * of the call (not by the lengths). */
+typedef struct msh_kv4_attention_args {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements; the last dimension is contiguous */
+  const int32_t* block_table; /* [batch][table_width] */
+  const int32_t* kv_lens;     /* [batch] */
+  const int32_t* q_start;     /* [batch + 1] or NULL */
+  msh_kv4_cache cache;
+  int64_t rows;
+  int32_t dtype, heads, batch, table_width, max_q, causal, window;
+  float scale;
+} msh_kv4_attention_args;
+MSH_EXPORT int64_t msh_kv4_attention_workspace(const msh_kv4_attention_args* args); /* bytes; may be 0 */
+MSH_EXPORT int32_t msh_kv4_attention(int32_t device, void* stream, const msh_kv4_attention_args* args, void* workspace,
+                                     int64_t workspace_bytes);
+
+/* One selection of a beam search.  Beam k of entry b has the accumulated log probability scores[b * beams + k] (-inf: not in use) and the
+ * logits at row (b * beams + k) * row_stride; its candidates are score + log_softmax(logits)[v] for every v with a logit above -inf.
+ * A finished beam (its logits are not read) has one candidate: itself, unchanged, with the token eos.  The `beams` best candidates of
+ * an entry, ties to the lowest beam * vocab + v, become its next beams: next_scores, parents (the beam each continues), tokens,
+ * next_finished (the parent was finished, or the token is eos).  Too few candidates: the rest are score -inf, parent = own index,
+ * token eos, finished.  eos = -1: no id ends a beam.  NaN logits count as -inf, +inf as the largest finite value.  1 to 16 beams.
+ * The outputs must not be the inputs. */
+MSH_EXPORT int64_t msh_beam_select_workspace(int32_t batch, int32_t beams, int32_t vocab);
+MSH_EXPORT int32_t msh_beam_select(int32_t device, void* stream, const void* logits, int32_t dtype, int64_t row_stride, int32_t batch,
+                                   int32_t beams, int32_t vocab, const float* scores, const uint8_t* finished, int32_t eos,
+                                   float* next_scores, int32_t* parents, int32_t* tokens, uint8_t* next_finished, void* workspace,
+                                   int64_t workspace_bytes);
+
+/* Reorder up to four states in place after a selection: the first min(length, n_rows) rows of beam k of entry b become those of beam
+ * parents[b * beams + k] (all at once: parents are the beams before the call).  A state is n_rows rows of row_bytes contiguous bytes for
+ * each (outer o, entry b, beam k, inner i), at data + o * outer_stride + (b * beams + k) * beam_stride + i * inner_stride: a cache
+ * [layers][entries * beams][heads][room][width] has outer = layers, inner = heads, row_bytes = width * size.  lengths: device int32, one
+ * per entry (length_stride 1) or one for all (0), NULL: n_rows.  A parent that is no beam leaves its child as it is.  The states and
+ * their rows must not overlap. */
+typedef struct msh_beam_state {
+  void* data;
+  int64_t outer, outer_stride, beam_stride, inner, inner_stride, row_bytes, n_rows; /* strides in bytes */
+} msh_beam_state;
+MSH_EXPORT int32_t msh_beam_reorder(int32_t device, void* stream, const msh_beam_state* states, int32_t n_states, int32_t batch,
+                                    int32_t beams, const int32_t* parents, const int32_t* lengths, int32_t length_stride);
+
+/* ---------------------------------------------------------------------------------------------------
  * Streaming models (reference core/moonshine-streaming-model.h:73-201).  One msh_stream_engine replaces the
  * five ORT sessions of MoonshineStreamingModel (frontend / encoder / adapter / cross_kv / decoder_kv) and
  * holds the per-stream state the reference keeps in MoonshineStreamingState (:36-71) on the device, one

@@ -111,6 +111,16 @@ def load_library(path: str | None = None) -> C.CDLL:
         "msh_host_sanitize_utf8": (C.c_int64, [vp, u64, vp, u64]),
         "msh_host_resample": (C.c_int64, [vp, u64, f32, f32, vp, u64]),
         "msh_set_hw_queues": (i32, [i32]),
+        "msh_op_last_error": (C.c_char_p, []),
+        "msh_page_plan": (i32, [i32, vp, vp, i32, i32, vp, vp, vp, C.c_int64, vp, C.c_int64, i32, vp, vp]),
+        "msh_kv4_page_bytes": (C.c_int64, [i32, i32, i32]),
+        "msh_kv4_write": (i32, [i32, vp, vp, vp, vp, vp, vp, i32, C.c_int64, vp]),
+        "msh_kv4_read": (i32, [i32, vp, vp, vp, C.c_int64, vp, vp, i32]),
+        "msh_kv4_attention_workspace": (C.c_int64, [vp]),
+        "msh_kv4_attention": (i32, [i32, vp, vp, vp, C.c_int64]),
+        "msh_beam_select_workspace": (C.c_int64, [i32, i32, i32]),
+        "msh_beam_select": (i32, [i32, vp, vp, i32, C.c_int64, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp, C.c_int64]),
+        "msh_beam_reorder": (i32, [i32, vp, vp, i32, i32, i32, vp, vp, i32]),
         "msh_host_load_wav": (C.c_int64, [C.c_char_p, vp, u64, vp]),
         "msh_host_save_wav": (i32, [C.c_char_p, vp, u64, i32]),
         "msh_host_silero_probabilities": (C.c_int64, [vp, u64, vp, u64, vp, u64, vp]),
@@ -178,6 +188,8 @@ DECLARED_SYMBOLS = [
     "msh_stream_profile_enable", "msh_stream_profile_reset", "msh_stream_profile_count", "msh_stream_profile_get",
     "msh_set_cross_mode", "msh_set_uniform_kernels", "msh_uniform_kernels", "msh_cross_absorbed", "msh_cross_absorbed_supported",
     "msh_stream_get_features",
+    "msh_op_last_error", "msh_page_plan", "msh_kv4_page_bytes", "msh_kv4_write", "msh_kv4_read", "msh_kv4_attention_workspace",
+    "msh_kv4_attention", "msh_beam_select_workspace", "msh_beam_select", "msh_beam_reorder",
 ]
 
 
