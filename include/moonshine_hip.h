@@ -111,9 +111,16 @@ MSH_EXPORT int32_t msh_get_encoder_output(msh_engine* e, uint32_t clip, float* o
 /* Storage of the cross-attention K / V the decoder streams every step (the `past_key_values.{l}.encoder.{key,value}` tensors
  * of the reference's decoder graph, core/moonshine-model.cpp:354-368, fp32 there): 0 = bf16 (default; the parity
  * tolerances of tests/ are stated for it), 1 = fp8 e4m3 with one scale per head-dim row fixed at load -- half the bytes of
- * the HBM-bound kernel that dominates a decode step; scores, softmax and accumulation stay fp32.  Applies from the next
- * msh_encode; call it before msh_set_batches_in_flight.  Not combinable with the cross-attention capture. */
+ * the HBM-bound kernel that dominates a decode step; scores, softmax and accumulation stay fp32; 2 = mxfp4, the paged 4-bit cache
+ * of the serving operators below: 4.25 bits an element (head widths padded to 32), read once for all beams of a clip.  Applies from
+ * the next msh_encode; call it before msh_set_batches_in_flight.  Not combinable with the cross-attention capture or the absorbed form. */
 MSH_EXPORT int32_t msh_set_kv_dtype(msh_engine* e, int32_t dtype);
+/* Beam search (additive; the reference decodes greedily, core/moonshine-model.cpp:454-470): msh_decode and what calls it keep `width`
+ * hypotheses per clip (1 to 16; 1 = greedy, the default) and return the one with the largest accumulated log probability divided by
+ * (number of generated ids, EOS included) ^ length_penalty.  With forced_steps >= 0 no id ends a hypothesis.  A teacher or logits_out
+ * is refused then, the cross-attention capture too.  Call it before msh_set_batches_in_flight. */
+MSH_EXPORT int32_t msh_set_beam_width(msh_engine* e, int32_t width, float length_penalty);
+MSH_EXPORT int32_t msh_beam_width(const msh_engine* e);
 
 /* Per-kernel-group timing with HIP events on the engine's stream (the role of the reference's
  * log_ort_run option, core/ort-utils/ort-utils.cpp:256-288).  While enabled the decode step runs

@@ -84,13 +84,16 @@ void apply_options(const OptionList& options, TranscriberOptions* o) {
     else if (k == "vad_device") o->vad_device = parse_int32(v);                    // additive: Silero on the GPU for batch calls
     else if (k == "host_threads") o->host_threads = parse_int32(v);                // additive: VAD threads of batch calls
     else if (k == "max_stream_seconds") o->max_stream_seconds = parse_float(v);     // additive (streaming archs)
-    else if (k == "kv_dtype") {   // additive: cross K / V on the device as bf16 (default) or fp8 e4m3
+    else if (k == "kv_dtype") {   // additive: cross K / V on the device as bf16 (default), fp8 e4m3 or mxfp4
       std::string t = v;
       for (char& ch : t) ch = (char)tolower((unsigned char)ch);
       if (t == "bf16") o->kv_dtype = 0;
       else if (t == "fp8" || t == "fp8_e4m3" || t == "e4m3") o->kv_dtype = 1;
-      else throw std::runtime_error("kv_dtype must be bf16 or fp8, got '" + v + "'");
+      else if (t == "mxfp4" || t == "fp4") o->kv_dtype = 2;   // the paged 4-bit cache of the serving operators
+      else throw std::runtime_error("kv_dtype must be bf16, fp8 or mxfp4, got '" + v + "'");
     }
+    else if (k == "beam_width") o->beam_width = parse_int32(v);                     // additive: hypotheses per clip (offline archs; msh_set_beam_width)
+    else if (k == "length_penalty") o->length_penalty = parse_float(v);             // additive: with beam_width > 1
     else if (k == "cross_attention") {   // additive: auto (default) | kv | absorbed (msh_set_cross_mode)
       std::string t = v;
       for (char& ch : t) ch = (char)tolower((unsigned char)ch);

@@ -1,5 +1,7 @@
 #include "engine.h"
 
+#include "serve_kernels.h"
+
 #include <atomic>
 
 #include "host_utils.h"
@@ -336,7 +338,8 @@ Engine::~Engine() {
     (void)hipEventDestroy(r.b);
   }
   DevBuf* bufs[] = {&clips_d_, &clip_ptrs_d_, &pcm_stage_, &audio_bf16_, &row_pos_, &row_clip_, &x1_, &x2_, &H_,
-                    &Y_, &QKV_, &VTe_, &AO_, &Z_, &ENC_, &ENC32_, &gn_part_, &gn_rows_, &gn_stats_, &gn_table_, &KT_, &VT_, &cross_probs_};
+                    &Y_, &QKV_, &VTe_, &AO_, &Z_, &ENC_, &ENC32_, &gn_part_, &gn_rows_, &gn_stats_, &gn_table_, &KT_, &VT_, &cross_probs_,
+                    &kv4_cache_, &kv4_rows_, &kv4_table_, &kv4_lens_, &kv4_slots_, &kv4_free_};
   for (DevBuf* b : bufs) b->release();
   if (pcm_pinned_) (void)hipHostFree(pcm_pinned_);
   if (stream_) (void)hipStreamDestroy(stream_);
@@ -432,7 +435,8 @@ void Engine::share_weights_from(const Engine& o) {
   cross_kv_panel_w_ = o.cross_kv_panel_w_;
   embed_f32_ = o.embed_f32_, dec_ln_ = o.dec_ln_;
   kv_qscale_ = o.kv_qscale_, kv_dq_ = o.kv_dq_;
-  kv_fp8_ = o.kv_fp8_;
+  kv_fp8_ = o.kv_fp8_, kv_dtype_ = o.kv_dtype_;
+  beam_width_ = o.beam_width_, length_penalty_ = o.length_penalty_;
   cross_mode_ = o.cross_mode_;
   uniform_kernels_ = o.uniform_kernels_;
   rope_cos_ = o.rope_cos_, rope_sin_ = o.rope_sin_;
@@ -961,14 +965,25 @@ void Engine::encode(const float* const* pcm, const uint64_t* n_samples, uint32_t
   // stays for small batches, for the word-timestamp capture (which reads K^T) and for fp8 keys.
   // The form is a property of the ENGINE (set_cross_mode), never of the batch: the same clip decodes to the same ids whatever
   // shares its batch.  (MSH_XATTN_MIN_BATCH=n restores the round-4 per-batch switch of mode 0 for A/B measurements only.)
-  if (cross_mode_ == 2 && (!cross_absorbed_available() || capture_cross_ || kv_fp8_))
+  if (cross_mode_ == 2 && (!cross_absorbed_available() || capture_cross_ || kv_dtype_ != 0))
     throw std::invalid_argument(std::string("cross_attention = absorbed cannot be honoured: ") +
                                 (!cross_absorbed_available() ? "this architecture has no absorbed operands"
                                  : capture_cross_            ? "the word-timestamp capture reads the projected keys"
-                                                             : "kv_dtype = fp8 stores projected keys"));
+                                                             : "kv_dtype = fp8 / mxfp4 stores projected keys"));
   absorbed_ = cross_mode_ == 2 || (cross_mode_ == 0 && xattn_min_batch() > 0 && cross_absorbed_available() && !capture_cross_ &&
-                                   !kv_fp8_ && (int)count >= xattn_min_batch());
-  if (!absorbed_) {
+                                   kv_dtype_ == 0 && (int)count >= xattn_min_batch());
+  if (kv_dtype_ == 2) {
+    int64_t pages = 0;
+    kv4_width_ = 0;
+    for (const ClipMeta& c : clips_h_) pages += (c.T + 31) / 32, kv4_width_ = std::max(kv4_width_, (c.T + 31) / 32);
+    kv4_pages_ = pages;
+    moved |= kv4_cache_.reserve((size_t)L * kv4_layer_bytes());
+    moved |= kv4_rows_.reserve((size_t)R * 2 * D * sizeof(bf16_t));
+    moved |= kv4_table_.reserve((size_t)count * kv4_width_ * sizeof(int32_t));
+    moved |= kv4_lens_.reserve(((size_t)2 * count + 1) * sizeof(int32_t));
+    moved |= kv4_slots_.reserve((size_t)R * sizeof(int64_t));
+    moved |= kv4_free_.reserve((size_t)pages * sizeof(int32_t));
+  } else if (!absorbed_) {
     moved |= KT_.reserve((size_t)L * D * kv_keys_ * kv_bytes());
     moved |= VT_.reserve((size_t)L * D * kv_keys_ * kv_bytes());
   }
@@ -1027,6 +1042,14 @@ void Engine::encode(const float* const* pcm, const uint64_t* n_samples, uint32_t
   }
   MSH_HIP(hipMemcpyAsync(clips_d_.p, clips_h_.data(), count * sizeof(ClipMeta), hipMemcpyHostToDevice, stream_));
   MSH_HIP(hipMemcpyAsync(clip_ptrs_d_.p, ptrs.data(), count * sizeof(float*), hipMemcpyHostToDevice, stream_));
+  std::vector<int32_t> kv4_meta, kv4_ids;
+  if (kv_dtype_ == 2) {   // frames and first row of every clip; every page is free
+    for (const ClipMeta& c : clips_h_) kv4_meta.push_back(c.T);
+    for (const ClipMeta& c : clips_h_) kv4_meta.push_back(c.row_start);
+    MSH_HIP(hipMemcpyAsync(kv4_lens_.p, kv4_meta.data(), kv4_meta.size() * sizeof(int32_t), hipMemcpyHostToDevice, stream_));
+    for (int64_t i = 0; i < kv4_pages_; ++i) kv4_ids.push_back((int32_t)i);
+    MSH_HIP(hipMemcpyAsync(kv4_free_.p, kv4_ids.data(), kv4_ids.size() * sizeof(int32_t), hipMemcpyHostToDevice, stream_));
+  }
   MSH_HIP(hipStreamSynchronize(stream_));  // `ptrs` / `clips_h_` staging is on the host stack
   if (upload_turn.owns_lock()) upload_turn.unlock();
   run_encoder();
@@ -1267,7 +1290,9 @@ void Engine::run_encoder() {
     ProfScope p(this, "enc_layernorm", 0, sT * D * 6);
     layernorm_bf16(H_.as<float>(), enc_ln_, R, D, ENC_.as<bf16_t>(), keep_enc_f32_ ? ENC32_.as<float>() : nullptr, s);
   }
-  if (!absorbed_) {  // cross-attention K/V of all decoder layers in one GEMM, written as K^T / V^T for the decode stream
+  if (kv_dtype_ == 2) {
+    write_kv4();
+  } else if (!absorbed_) {  // cross-attention K/V of all decoder layers in one GEMM, written as K^T / V^T for the decode stream
     // The panel kernel's cross-KV instance is OFF unless asked for (MSH_ENC_CROSS_KV_PANEL=2): at 256 x 10 s it measured
     // 1.01 ms against 0.93 ms for the A-stationary tiled kernel -- this GEMM writes 1.42 GB of K^T / V^T per batch and is
     // bound by that, not by its operand traffic.  Its parity test keeps the instance honest.
@@ -1283,6 +1308,38 @@ void Engine::run_encoder() {
     else
       gemm_cross_kv(ENC_.as<bf16_t>(), D, cross_kv_w_, R, L * 2 * D, D, row_clip_.as<int>(), clips, D,
                     (long)D * kv_keys_, KT_.as<bf16_t>(), VT_.as<bf16_t>(), s);
+  }
+}
+
+// ---- cross K / V in the paged 4-bit cache (kv_dtype = mxfp4; serve_kernels.h) ----
+static Kv4Cache kv4_cache_of(void* p, int64_t pages, int heads, int dh) { return Kv4Cache{static_cast<uint8_t*>(p), pages, heads, 5, dh}; }
+
+size_t Engine::kv4_layer_bytes() const {
+  return (size_t)kv4_pages_ * cfg_.heads * kv4_block_bytes(kv4_groups(cfg_.head_dim()));
+}
+
+// One plan for all layers, then layer by layer the projection (row-major bf16, one buffer for all layers) and the rows into their slots.
+// The rows of a batch are clips padded to 8 rows: the plan gives padding the slot -1.
+void Engine::write_kv4() {
+  const int D = cfg_.hidden, Hh = cfg_.heads, dh = cfg_.head_dim(), L = cfg_.dec_layers, n = (int)n_clips_;
+  double sT = 0;
+  for (const ClipMeta& c : clips_h_) sT += c.T;
+  hipStream_t s = stream_;
+  const int32_t* lens = kv4_lens_.as<int32_t>();
+  {
+    ProfScope p(this, "cross_kv4_plan", 0, R_ * 8.0 + n * (kv4_width_ + 3) * 4.0);
+    page_plan(kv4_table_.as<int32_t>(), n, kv4_width_, lens, lens, lens + n, R_, kv4_free_.as<int32_t>(), kv4_pages_, 5,
+              kv4_slots_.as<int64_t>(), kv4_lens_.as<int32_t>() + 2 * n, s);
+  }
+  bf16_t* rows = kv4_rows_.as<bf16_t>();
+  for (int l = 0; l < L; ++l) {
+    {
+      ProfScope p(this, "cross_kv_gemm", 2.0 * sT * D * 2 * D, sT * D * 2 + sT * D * 4.0 + 4.0 * D * D);
+      gemm_act(ENC_.as<bf16_t>(), D, cross_kv_w_ + (size_t)l * 2 * D * D, nullptr, 0, (int)R_, 2 * D, D, rows, nullptr, s);
+    }
+    ProfScope p(this, "cross_kv4_write", 0, sT * D * 4.0 + sT * Hh * 34.0 * kv4_groups(dh));
+    kv4_write(kv4_cache_of(kv4_cache_.as<char>() + l * kv4_layer_bytes(), kv4_pages_, Hh, dh), Kv4Rows{rows, 2 * D, dh, 1},
+              Kv4Rows{rows + D, 2 * D, dh, 1}, Elem::bf16, R_, kv4_slots_.as<int64_t>(), s);
   }
 }
 
@@ -1310,6 +1367,8 @@ struct Engine::DecodeGroup {
   bool own_stream = false;
   int first = 0, M = 0;
   DevBuf dH, dq, dao, dz, dy, logits, cacheK, cacheV, tokens, counts, finished, scalars, teacher, pval, pidx, xpart;
+  int beams = 1;              // rows of a clip (row = clip * beams + beam); > 1: row_clips holds every row's clip
+  DevBuf row_clips, scores, beam_out, beam_work, kv4_part;
   bool self_fused = false;    // single-clip latency path: self-attention inside the output projection's launch (<= 2 clips)
   bool loop_cross = false;    // 5 .. 63 clips: the same cross-attention with one workgroup per (clip, head) walking the slices
   bool split_cross = false;   // single-clip latency path: cross-attention split over key slices (k_dec_small.hip)
@@ -1347,7 +1406,7 @@ struct Engine::DecodeGroup {
   ~DecodeGroup() {
     drop_graphs();
     DevBuf* bufs[] = {&dH, &dq, &dao, &dz, &dy, &logits, &cacheK, &cacheV, &tokens, &counts, &finished, &scalars, &teacher,
-                      &pval, &pidx, &xpart};
+                      &pval, &pidx, &xpart, &row_clips, &scores, &beam_out, &beam_work, &kv4_part};
     for (DevBuf* b : bufs) b->release();
     if (own_stream && stream) (void)hipStreamDestroy(stream);
   }
@@ -1359,6 +1418,7 @@ double Engine::profile_cross_attention_ms(int rounds) {
   MSH_HIP(hipSetDevice(device_));
   if (!encoded_ || groups_.empty() || groups_[0]->M != (int)n_clips_)
     throw std::runtime_error("profile_cross_attention: encode and decode a batch first");
+  if (groups_[0]->beams > 1) throw std::runtime_error("profile_cross_attention: decode the batch greedily first");
   // rounds < 0 (probe): every launch reads layer 0's K / V again -- one layer of a 256-clip batch is 177 MB, inside the
   // 256 MB memory-side cache, so this is the kernel's rate when its operands do NOT come from HBM
   const bool same_layer = rounds < 0;
@@ -1373,6 +1433,10 @@ double Engine::profile_cross_attention_ms(int rounds) {
       const int ll = same_layer ? 0 : l;
       if (absorbed_) {   // every layer reads the same encoder output (that IS the decode step's access pattern)
         dec_cross_absorbed(g.dq.as<bf16_t>(), ENC_.as<bf16_t>(), clips_d_.as<ClipMeta>(), g.M, D, cfg_.heads, g.dao.as<bf16_t>(), stream_);
+        continue;
+      }
+      if (kv_dtype_ == 2) {
+        kv4_attend(g, ll, stream_);
         continue;
       }
       dec_cross_attention(g.dq.as<float>(), kv_layer(KT_, ll), kv_layer(VT_, ll), clips_d_.as<ClipMeta>(), g.M, D, cfg_.heads,
@@ -1395,7 +1459,7 @@ double Engine::profile_cross_attention_ms(int rounds) {
 size_t Engine::debug_read(const std::string& name, void* dst, size_t bytes) {
   MSH_HIP(hipSetDevice(device_));
   if (name == "cross_k" || name == "cross_v") {   // K^T / V^T of the last encode(): [layers][D * keys] at kv_bytes() per key
-    if (absorbed_) throw std::runtime_error("debug_read: the last batch used the absorbed cross-attention, K^T / V^T were not written");
+    if (absorbed_ || kv_dtype_ == 2) throw std::runtime_error("debug_read: the last batch's cross-attention form wrote no K^T / V^T");
     const size_t size = (size_t)cfg_.dec_layers * cfg_.hidden * kv_keys_ * kv_bytes();
     MSH_HIP(hipStreamSynchronize(stream_));
     if (dst != nullptr && bytes > 0) copy_blocking(dst, name == "cross_k" ? KT_.p : VT_.p, std::min(bytes, size), hipMemcpyDeviceToHost);
@@ -1448,10 +1512,10 @@ void Engine::decode_step_enqueue(DecodeGroup& g) {
   float* dq = g.dq.as<float>();
   bf16_t* dao = g.dao.as<bf16_t>();
   bf16_t* dz = g.dz.as<bf16_t>();
-  const ClipMeta* clips = clips_d_.as<ClipMeta>() + g.first;
+  const ClipMeta* clips = g.beams > 1 ? g.row_clips.as<ClipMeta>() : clips_d_.as<ClipMeta>() + g.first;
   const size_t cache_layer = (size_t)M * Hh * Smax_ * dh;
   double sT = 0;
-  for (int b = 0; b < M; ++b) sT += clips_h_[g.first + b].T;
+  for (int b = 0; b < M; ++b) sT += clips_h_[g.first + b / g.beams].T;
   const double w_dd = 2.0 * D * D;  // bytes of a [D, D] bf16 weight
   dec_gemm_prefer_throughput(shared_gpu_ && M >= 192);
   // chain profiling (profile_decode_chain): enqueue only the kernel group `step_only_`
@@ -1524,6 +1588,15 @@ void Engine::decode_step_enqueue(DecodeGroup& g) {
         ProfScope p(this, "dec_cross_attention", 4.0 * sT * D + 2.0 * M * D * D, sT * D * 2.0 * kv_bytes() + w_dd + M * D * 4.0);
         dec_cross_looped(dH, W.wq_c_rm, KTl, VTl, clips, M, D, Hh, dao, s);
       }
+    } else if (kv_dtype_ == 2) {
+      if (on(3)) {
+        ProfScope p(this, "dec_crossq_gemm", 2.0 * M * D * D, w_dd + M * D * 8.0);
+        dec_gemm_ln_f32(dH, W.wq_c, M, D, D, dq, s);
+      }
+      if (on(4)) {   // a clip's cache is read once for all its beams
+        ProfScope p(this, "dec_cross_attention", 4.0 * sT * D, sT / g.beams * Hh * 68.0 * kv4_groups(dh) / 2 + M * D * 6.0);
+        kv4_attend(g, l, s);
+      }
     } else if (fuse_q && D <= 512 && M < 64 && !capture_cross_ && !uniform_kernels_) {  // latency-bound regime only (see k_attn.hip)
       // LayerNorm + query projection of the clip's row run inside the attention kernel
       if (on(4)) {
@@ -1574,6 +1647,25 @@ void Engine::decode_step_enqueue(DecodeGroup& g) {
     ProfScope p(this, "dec_lm_head_gemm", 2.0 * M * D * V, 2.0 * V * D + M * (double)V * 4);
     dec_gemm_logits(dH, embed_head_folded_, M, V, D, g.logits.as<float>(), s);
   }
+}
+
+void Engine::kv4_attend(DecodeGroup& g, int layer, hipStream_t s) {
+  const int D = cfg_.hidden, dh = cfg_.head_dim();
+  Kv4Attention a{};
+  a.q = g.dq.p;
+  a.q_row = D, a.q_head = dh;
+  a.fm = g.dao.as<uint16_t>();
+  a.table = kv4_table_.as<int32_t>() + (size_t)g.first * kv4_width_;
+  a.kv_lens = kv4_lens_.as<int32_t>() + g.first;
+  a.cache = kv4_cache_of(kv4_cache_.as<char>() + layer * kv4_layer_bytes(), kv4_pages_, cfg_.heads, dh);
+  a.rows = g.M, a.heads = cfg_.heads, a.batch = g.M / g.beams, a.width = kv4_width_, a.max_q = g.beams;
+  a.scale_log2 = 1.44269504088896341f / sqrtf((float)dh);
+  // (one kernel set for every call: the order of a clip's sums must not go by what shares its call)
+  a.nsplit = uniform_kernels_ ? 1 : kv4_attention_splits(a, Elem::f32);
+  const size_t need = kv4_attention_part_floats(a, a.nsplit) * sizeof(float);
+  if (need > g.kv4_part.cap) throw std::runtime_error("kv4_attend: workspace not reserved");
+  a.part = g.kv4_part.as<float>();
+  kv4_attention(a, Elem::f32, s);
 }
 
 // Per-launch cost of every decode kernel group INSIDE a dependent chain of a replayed hipGraph -- the way the decode
@@ -1710,6 +1802,10 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
   if (!encoded_) throw std::runtime_error("decode() called before encode()");
   const int Mtot = (int)n_clips_, D = cfg_.hidden, F = cfg_.ffn, V = cfg_.vocab, Hh = cfg_.heads, dh = cfg_.head_dim();
   const bool forced = forced_steps >= 0;
+  if (beam_width_ > 1) {
+    if (teacher != nullptr || logits_out != nullptr) throw std::invalid_argument("decode: a beam search takes no teacher and returns no logits");
+    return decode_beams(forced_steps, tokens_out, counts_out, tokens_stride);
+  }
   const int steps = forced ? forced_steps : max_steps_;
   if (steps < 1) throw std::invalid_argument("decode: need at least one step");
   if (steps > 504) throw std::invalid_argument("decode: step budget above 504 tokens is not supported");
@@ -1763,6 +1859,7 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
   std::vector<DecodeState> states(ngroups);
   for (int gi = 0; gi < ngroups; ++gi) {
     DecodeGroup& g = *groups_[gi];
+    g.beams = 1;
     g.first = (int)((long)Mtot * gi / ngroups);
     g.M = (int)((long)Mtot * (gi + 1) / ngroups) - g.first;
     const int M = g.M;
@@ -1796,7 +1893,7 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
       int tmax = 1;
       for (int b = 0; b < M; ++b) tmax = std::max(tmax, (int)clips_h_[g.first + b].T);
       const int xs = dec_cross_split_slices(tmax);
-      const bool small_ok = !uniform_kernels_ && !absorbed_ && !capture_cross_ && !kv_fp8_ && M < 64 && dec_cross_split_supported(D, Hh);
+      const bool small_ok = !uniform_kernels_ && !absorbed_ && !capture_cross_ && kv_dtype_ == 0 && M < 64 && dec_cross_split_supported(D, Hh);
       g.split_cross = small_ok && M <= xsplit_m;
       const char* xl = dev_getenv("MSH_XLOOP");   // 0: batches above MSH_XSPLIT_M keep k_attn.hip's one-pass kernel (A/B measurements)
       g.loop_cross = small_ok && !g.split_cross && xs <= dec_cross_looped_max_slices() && !(xl != nullptr && xl[0] == '0');
@@ -1806,6 +1903,7 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
         moved |= g.xpart.reserve(dec_cross_split_part_floats(M, Hh, xs) * sizeof(float));
       }
     }
+    if (kv_dtype_ == 2) moved |= g.kv4_part.reserve(kv4_part_bytes(M, 1));
     moved |= g.cacheK.reserve((size_t)cfg_.dec_layers * M * Hh * Smax_ * dh * sizeof(bf16_t));
     moved |= g.cacheV.reserve((size_t)cfg_.dec_layers * M * Hh * Smax_ * dh * sizeof(bf16_t));
     moved |= g.tokens.reserve((size_t)M * dstride * sizeof(int32_t));
@@ -1840,7 +1938,7 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
       const std::string key = std::to_string(M) + ":" + std::to_string(g.first) + ":" + std::to_string(Smax_) + ":" +
                               std::to_string(st.ignore_eos) + ":" + std::to_string(teacher != nullptr) + ":" +
                               std::to_string(absorbed_ ? 0 : kv_keys_) + ":" + std::to_string(g.fused_argmax) + ":" +
-                              std::to_string(kv_fp8_) + ":" + std::to_string(absorbed_) + ":" + std::to_string(g.split_cross ? g.xs_max : 0) + ":" + std::to_string(g.self_fused) + ":" + std::to_string(g.loop_cross);
+                              std::to_string(kv_dtype_) + ":" + (kv_dtype_ == 2 ? std::to_string(kv4_pages_) + "," + std::to_string(kv4_width_) + "," + std::to_string(uniform_kernels_) : std::string()) + ":" + std::to_string(absorbed_) + ":" + std::to_string(g.split_cross ? g.xs_max : 0) + ":" + std::to_string(g.self_fused) + ":" + std::to_string(g.loop_cross);
       if (g.graphs_ws_gen != ws_gen_ || g.graphs_gen != g.gen) {   // a workspace moved: every captured pointer is stale
         g.drop_graphs();
         g.graphs_ws_gen = ws_gen_, g.graphs_gen = g.gen;
@@ -1981,6 +2079,168 @@ int Engine::decode(int forced_steps, const int32_t* teacher, int teacher_stride,
       MSH_HIP(hipMemcpyAsync(cross_counts_.data() + g.first, g.counts.p, (size_t)g.M * sizeof(int32_t), hipMemcpyDeviceToHost, g.stream));
       MSH_HIP(hipStreamSynchronize(g.stream));
     }
+  }
+  prof_flush();
+  return steps_run;
+}
+
+size_t Engine::kv4_part_bytes(int rows, int beams) const {
+  Kv4Attention a{};
+  a.cache = kv4_cache_of(nullptr, kv4_pages_, cfg_.heads, cfg_.head_dim());
+  a.rows = rows, a.heads = cfg_.heads, a.batch = rows / beams, a.width = kv4_width_, a.max_q = beams;
+  return std::max((size_t)16, kv4_attention_part_floats(a, kv4_attention_splits(a, Elem::f32)) * sizeof(float));
+}
+
+// Beam search over the encoded batch, lock-step: every clip has beam_width_ rows.  A step is the greedy loop's step over all rows, then the
+// selection over beams and vocabulary, the reordering of the self-attention caches and of the ids, and the bookkeeping -- all on the device,
+// replayed from one captured graph; the host looks at the number of clips still decoding every eighth step.
+int Engine::decode_beams(int forced_steps, int32_t* tokens_out, int32_t* counts_out, int tokens_stride) {
+  const int K = beam_width_, n = (int)n_clips_, M = n * K, D = cfg_.hidden, F = cfg_.ffn, V = cfg_.vocab, Hh = cfg_.heads, dh = cfg_.head_dim();
+  const int L = cfg_.dec_layers;
+  const bool forced = forced_steps >= 0;
+  const int steps = forced ? forced_steps : max_steps_;
+  if (steps < 1) throw std::invalid_argument("decode: need at least one step");
+  if (steps > 504) throw std::invalid_argument("decode: step budget above 504 tokens is not supported");
+  if (tokens_out != nullptr && tokens_stride < steps + 1)
+    throw std::invalid_argument("decode: tokens_stride " + std::to_string(tokens_stride) + " < steps+1 = " + std::to_string(steps + 1));
+  if ((long)n * K > 65535) throw std::invalid_argument("decode: clips * beam_width above 65535");
+  Smax_ = steps <= 72 ? 72 : steps <= 144 ? 144 : steps <= 288 ? 288 : 512;   // capacity buckets, as in decode()
+  const int dstride = Smax_ + 8;
+  if (groups_.empty()) {
+    std::unique_ptr<DecodeGroup> g0(new DecodeGroup());
+    g0->stream = stream_;
+    groups_.push_back(std::move(g0));
+  }
+  DecodeGroup& g = *groups_[0];
+  hipStream_t s = g.stream;
+  g.first = 0, g.M = M, g.beams = K;
+  g.fused_argmax = g.self_fused = g.loop_cross = g.split_cross = false;
+  bool moved = false;
+  const size_t M16 = (size_t)round_up(M, 16);
+  const int xw = absorbed_ ? Hh : 1;
+  const size_t cache_bytes = (size_t)L * M * Hh * Smax_ * dh * sizeof(bf16_t);
+  moved |= g.dH.reserve(M16 * D * sizeof(float));
+  moved |= g.dq.reserve((size_t)M * D * xw * sizeof(float));
+  moved |= g.dao.reserve(M16 * D * xw * sizeof(bf16_t));
+  moved |= g.dz.reserve(M16 * F * sizeof(bf16_t));
+  moved |= g.dy.reserve((size_t)M * D * sizeof(bf16_t));
+  moved |= g.logits.reserve((size_t)M * V * sizeof(float));
+  moved |= g.cacheK.reserve(cache_bytes);
+  moved |= g.cacheV.reserve(cache_bytes);
+  moved |= g.tokens.reserve((size_t)M * dstride * sizeof(int32_t));
+  moved |= g.finished.reserve((size_t)M * 2);                             // flags, next flags
+  moved |= g.scalars.reserve(16 * sizeof(int32_t));
+  moved |= g.scores.reserve((size_t)M * 2 * sizeof(float));               // scores, next scores
+  moved |= g.beam_out.reserve((size_t)M * 2 * sizeof(int32_t));           // parents, ids
+  moved |= g.beam_work.reserve(beam_select_work_bytes(n, K, V));
+  moved |= g.row_clips.reserve((size_t)M * sizeof(ClipMeta));
+  if (kv_dtype_ == 2) moved |= g.kv4_part.reserve(kv4_part_bytes(M, K));
+  if (moved) ++g.gen;
+  std::vector<ClipMeta> rows((size_t)M);
+  for (int r = 0; r < M; ++r) {
+    rows[r] = clips_h_[r / K];
+    if (forced) rows[r].max_len = steps;
+  }
+  MSH_HIP(hipMemcpyAsync(g.row_clips.p, rows.data(), rows.size() * sizeof(ClipMeta), hipMemcpyHostToDevice, s));
+  MSH_HIP(hipStreamSynchronize(s));
+
+  BeamLoop loop{g.tokens.as<int32_t>(), g.scalars.as<int32_t>(), g.scores.as<float>(), g.scores.as<float>() + M, g.finished.as<uint8_t>(),
+                g.finished.as<uint8_t>() + M, g.beam_out.as<int32_t>(), g.beam_out.as<int32_t>() + M, dstride, K, n};
+  const BeamSelect pick{g.logits.p, V, loop.scores, loop.finished, loop.next_scores, g.beam_out.as<int32_t>(), g.beam_out.as<int32_t>() + M,
+                        loop.next_finished, g.beam_work.p, n, K, V, forced ? -1 : cfg_.eos};
+  const int64_t head = (int64_t)Smax_ * dh * sizeof(bf16_t);
+  const BeamState states[3] = {
+      {g.cacheK.p, L, (int64_t)M * Hh * head, Hh * head, Hh, head, (int64_t)(dh * sizeof(bf16_t)), Smax_},
+      {g.cacheV.p, L, (int64_t)M * Hh * head, Hh * head, Hh, head, (int64_t)(dh * sizeof(bf16_t)), Smax_},
+      {g.tokens.p, 1, 0, (int64_t)dstride * (int64_t)sizeof(int32_t), 1, 0, sizeof(int32_t), dstride},
+  };
+  auto step = [&] {
+    decode_step_enqueue(g);
+    {
+      ProfScope p(this, "dec_beam_select", 0, (double)M * V * 4);
+      beam_select(pick, Elem::f32, s);
+    }
+    {
+      ProfScope p(this, "dec_beam_reorder", 0, 0);
+      beam_reorder(states, 3, n, K, loop.parents, g.scalars.as<int32_t>() + 2, 0, s);
+    }
+    ProfScope p(this, "dec_beam_advance", 0, (double)M * D * 8);
+    beam_advance(loop, g.row_clips.as<ClipMeta>(), embed_f32_, D, g.dH.as<float>(), s);
+  };
+  beam_begin(loop, cfg_.bos, embed_f32_, D, g.dH.as<float>(), s);
+  const bool eager = prof_on_ || !use_graph_;
+  hipGraphExec_t graph = nullptr;
+  if (!eager) {
+    const std::string key = "beams:" + std::to_string(K) + ":" + std::to_string(n) + ":" + std::to_string(Smax_) + ":" + std::to_string(forced) + ":" +
+                            std::to_string(absorbed_ ? 0 : kv_keys_) + ":" + std::to_string(kv_dtype_) + ":" + std::to_string(kv4_pages_) + ":" +
+                            std::to_string(kv4_width_) + ":" + std::to_string(absorbed_) + ":" + std::to_string(uniform_kernels_);
+    if (g.graphs_ws_gen != ws_gen_ || g.graphs_gen != g.gen) {
+      g.drop_graphs();
+      g.graphs_ws_gen = ws_gen_, g.graphs_gen = g.gen;
+    }
+    DecodeGroup::GraphEntry* ent = nullptr;
+    for (DecodeGroup::GraphEntry& ge : g.graphs)
+      if (ge.key == key) ent = &ge;
+    if (ent == nullptr) {
+      if (g.graphs.size() >= DecodeGroup::kGraphCache) g.drop_graphs();
+      hipGraph_t gr = nullptr;
+      hipGraphExec_t exec = nullptr;
+      std::lock_guard<std::mutex> structure_lock(device_structure_mutex(device_));
+      MSH_HIP(hipStreamBeginCapture(s, hipStreamCaptureModeThreadLocal));
+      try {
+        step();
+      } catch (...) {
+        (void)hipStreamEndCapture(s, &gr);
+        if (gr != nullptr) (void)hipGraphDestroy(gr);
+        throw;
+      }
+      MSH_HIP(hipStreamEndCapture(s, &gr));
+      const hipError_t inst = hipGraphInstantiate(&exec, gr, nullptr, nullptr, 0);
+      (void)hipGraphDestroy(gr);
+      MSH_HIP(inst);
+      ++g.captures;
+      g.graphs.emplace_back();
+      ent = &g.graphs.back();
+      ent->key = key;
+      ent->g1 = exec;
+    }
+    ++ent->uses;
+    ent->last = ++g.graph_clock;
+    graph = ent->g1;
+  }
+  g.has_state = false;   // (the profiler's chains replay a greedy step)
+  int steps_run = 0;
+  for (int i = 0; i < steps; ++i) {
+    if (eager) step();
+    else MSH_HIP(hipGraphLaunch(graph, s));
+    ++steps_run;
+    if (!forced && (i & 7) == 7 && i + 1 < steps) {
+      int32_t active = 0;
+      MSH_HIP(hipMemcpyAsync(&active, g.scalars.as<int32_t>() + 1, sizeof(int32_t), hipMemcpyDeviceToHost, s));
+      MSH_HIP(hipStreamSynchronize(s));
+      if (active <= 0) break;
+    }
+  }
+  std::vector<int32_t> ids((size_t)M * dstride);
+  std::vector<float> scores((size_t)M);
+  MSH_HIP(hipMemcpyAsync(ids.data(), g.tokens.p, ids.size() * sizeof(int32_t), hipMemcpyDeviceToHost, s));
+  MSH_HIP(hipMemcpyAsync(scores.data(), loop.scores, scores.size() * sizeof(float), hipMemcpyDeviceToHost, s));
+  MSH_HIP(hipStreamSynchronize(s));
+  for (int c = 0; c < n; ++c) {
+    int best = 0, best_len = 0;
+    double best_score = -INFINITY;
+    for (int k = 0; k < K; ++k) {
+      const int32_t* t = ids.data() + (size_t)(c * K + k) * dstride;
+      int len = 0;   // generated ids
+      while (len < steps_run && t[len + 1] >= 0) ++len;
+      if (len == 0 || !(scores[(size_t)c * K + k] > -INFINITY)) continue;
+      const double v = (double)scores[(size_t)c * K + k] / pow((double)len, (double)length_penalty_);
+      if (best_len == 0 || v > best_score) best = k, best_len = len, best_score = v;
+    }
+    const int32_t* t = ids.data() + (size_t)(c * K + best) * dstride;
+    if (counts_out) counts_out[c] = best_len + 1;
+    if (tokens_out)
+      for (int i = 0; i < tokens_stride; ++i) tokens_out[(size_t)c * tokens_stride + i] = i <= best_len ? t[i] : -1;
   }
   prof_flush();
   return steps_run;

@@ -92,7 +92,8 @@ class Engine {
   // fp32 block (steps = tokens generated, T = encoder frames) to `out` if it holds `cap` >= that many floats, and
   // returns the three dimensions.
   void set_capture_cross_attention(bool on) {
-    if (on && kv_fp8_) throw std::invalid_argument("cross-attention capture (word timestamps) needs kv_dtype = bf16");
+    if (on && kv_dtype_ != 0) throw std::invalid_argument("cross-attention capture (word timestamps) needs kv_dtype = bf16");
+    if (on && beam_width_ > 1) throw std::invalid_argument("cross-attention capture (word timestamps) needs a greedy decode (beam_width = 1)");
     if (on && absorbed_) encoded_ = false;   // the capture reads K^T, which the absorbed form never writes: encode again
     capture_cross_ = on;
   }
@@ -130,15 +131,27 @@ class Engine {
   // go with the non-temporal policy (kernels.h dec_cross_absorbed)
   void set_shared_gpu(bool on) { shared_gpu_ = on; }
   bool cross_absorbed() const { return absorbed_; }   // of the batch encoded last
-  // cross K^T / V^T storage: bf16 (default) or e4m3 bytes with per-column scales fixed at load; applies to the next encode.
-  // Lanes (batches in flight) take the setting when they are created.
-  void set_kv_fp8(bool on) {
-    if (on && capture_cross_) throw std::invalid_argument("kv_dtype = fp8 cannot be combined with the cross-attention capture");
-    if (on != kv_fp8_) {
-      kv_fp8_ = on;
+  // storage of the cross K / V: 0 = bf16 K^T / V^T (default), 1 = the same as e4m3 bytes with per-column scales fixed at load,
+  // 2 = the paged 4-bit cache of the serving operators (serve_kernels.h), a page table per clip built on the device; applies to
+  // the next encode.  Lanes (batches in flight) take the setting when they are created.
+  void set_kv_dtype(int dtype) {
+    if (dtype < 0 || dtype > 2) throw std::invalid_argument("kv dtype: 0 = bf16, 1 = fp8 (e4m3), 2 = mxfp4");
+    if (dtype != 0 && capture_cross_) throw std::invalid_argument("kv_dtype = fp8 / mxfp4 cannot be combined with the cross-attention capture");
+    if (dtype != kv_dtype_) {
+      kv_dtype_ = dtype;
+      kv_fp8_ = dtype == 1;
       encoded_ = false;
     }
   }
+  // Beam search: decode() keeps `width` hypotheses per clip (1 = greedy, the default) and returns the one with the best accumulated
+  // log probability / (generated ids)^length_penalty.  Not combinable with teacher forcing, logits or the cross-attention capture.
+  void set_beam_width(int width, float length_penalty) {
+    if (width < 1 || width > 16) throw std::invalid_argument("beam width: 1 to 16");
+    if (!(length_penalty >= -8.f && length_penalty <= 8.f)) throw std::invalid_argument("length penalty: -8 to 8");
+    if (width > 1 && capture_cross_) throw std::invalid_argument("beam_width > 1 cannot be combined with the cross-attention capture");
+    beam_width_ = width, length_penalty_ = length_penalty;
+  }
+  int beam_width() const { return beam_width_; }
   bool kv_fp8() const { return kv_fp8_; }
   void get_cross_attention(uint32_t clip, float* out, size_t cap, int dims[3]);
 
@@ -209,7 +222,19 @@ class Engine {
   int max_rows_ = 0, max_steps_ = 0;
   bool encoded_ = false, keep_enc_f32_ = false;
   bool capture_cross_ = false;
-  bool kv_fp8_ = false;
+  bool kv_fp8_ = false;     // kv_dtype_ == 1
+  int kv_dtype_ = 0;
+  int beam_width_ = 1;
+  float length_penalty_ = 1.f;
+  // kv_dtype_ 2: per layer a cache of kv4_pages_ pages of 32 tokens; one table and slot map for all layers
+  int64_t kv4_pages_ = 0;
+  int kv4_width_ = 0;       // pages of the longest clip
+  size_t kv4_layer_bytes() const;
+  DevBuf kv4_cache_, kv4_rows_, kv4_table_, kv4_lens_, kv4_slots_, kv4_free_;
+  void write_kv4();         // page table and slot map of the batch, K / V of all layers
+  size_t kv4_part_bytes(int rows, int beams) const;
+  void kv4_attend(DecodeGroup& g, int layer, hipStream_t s);
+  int decode_beams(int forced_steps, int32_t* tokens_out, int32_t* counts_out, int tokens_stride);
   int cross_mode_ = 0;
   bool uniform_kernels_ = false;
   bool shared_gpu_ = false;

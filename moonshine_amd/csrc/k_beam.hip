@@ -1,6 +1,7 @@
 // Beam search: selection over beams and vocabulary, reordering of the states that the selected beams continue.
 #include <float.h>
 
+#include "kernels.h"
 #include "kv4_common.h"
 
 namespace msh {
@@ -336,7 +337,60 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamStates all, int n
   else move_piece<KMAX, uint8_t>(p + o, s.beam_stride, par, beams, 1);
 }
 
+// ---- the decode loop ----------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(128) void beam_begin_kernel(BeamLoop l, int bos, const float* __restrict__ embed, int D, float* __restrict__ H) {
+  const int row = blockIdx.x;
+  if (threadIdx.x == 0) {
+    l.tokens[(int64_t)row * l.stride] = bos;
+    l.scores[row] = row % l.beams == 0 ? 0.f : -INFINITY;   // all beams grow from one
+    l.finished[row] = 0;
+    if (row == 0) l.pos[0] = 0, l.pos[1] = l.clips, l.pos[2] = 1;
+  }
+  for (int d = threadIdx.x; d < D; d += 128) H[fm32(row, d, D >> 5)] = embed[(int64_t)bos * D + d];
+}
+
+// one workgroup per clip: its beams' old flags are read before any is written
+__global__ __launch_bounds__(256) void beam_advance_kernel(BeamLoop l, const ClipMeta* __restrict__ row_clips, const float* __restrict__ embed,
+                                                           int D, float* __restrict__ H) {
+  __shared__ uint8_t was_s[kBeamMax], now_s[kBeamMax];
+  const int row0 = blockIdx.x * l.beams, k = threadIdx.x, pos = l.pos[0];
+  if (k < l.beams) was_s[k] = l.finished[row0 + k];
+  __syncthreads();
+  if (k < l.beams) {
+    const int row = row0 + k;
+    const bool over = was_s[l.parents[row]] != 0;
+    l.tokens[(int64_t)row * l.stride + pos + 1] = over ? -1 : l.picked[row];
+    now_s[k] = l.next_finished[row] != 0 || pos + 1 >= row_clips[row].max_len;
+    l.finished[row] = now_s[k];
+    l.scores[row] = l.next_scores[row];
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    bool was = true, now = true;
+    for (int i = 0; i < l.beams; ++i) was = was && was_s[i] != 0, now = now && now_s[i] != 0;
+    if (now && !was) atomicSub(l.pos + 1, 1);
+  }
+  for (int i = threadIdx.x; i < l.beams * D; i += 256) {
+    const int row = row0 + i / D, d = i % D;
+    const int id = l.picked[row];
+    H[fm32(row, d, D >> 5)] = embed[(int64_t)(id < 0 ? 0 : id) * D + d];
+  }
+}
+
+__global__ void beam_tick_kernel(int32_t* pos) {
+  pos[0] += 1;
+  pos[2] += 1;
+}
+
 }  // namespace
+
+void beam_begin(const BeamLoop& l, int bos, const float* embed, int D, float* H, hipStream_t s) {
+  MSH_LAUNCH(beam_begin_kernel, dim3(l.clips * l.beams), dim3(128), 0, s, l, bos, embed, D, H);
+}
+void beam_advance(const BeamLoop& l, const ClipMeta* row_clips, const float* embed, int D, float* H, hipStream_t s) {
+  MSH_LAUNCH(beam_advance_kernel, dim3(l.clips), dim3(256), 0, s, l, row_clips, embed, D, H);
+  MSH_LAUNCH(beam_tick_kernel, dim3(1), dim3(1), 0, s, l.pos);
+}
 
 size_t beam_select_work_bytes(int batch, int beams, int vocab) {
   return (size_t)batch * beams * beam_parts(batch, beams, vocab) * part_bytes(beams);

@@ -17,6 +17,7 @@
 // the common block needs no cross-lane step and no rescaling; p <= 2^8 keeps its relative precision.
 #pragma once
 
+#include "kernels.h"
 #include "kv4_common.h"
 
 namespace msh {
@@ -343,6 +344,12 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
       return;
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    if (a.fm != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (d0 + e < a.cache.head_dim) a.fm[fm16((int)row, h * a.cache.head_dim + d0 + e, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(v[e] * inv);
+      return;
+    }
     T* o = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + d0;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -434,7 +441,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   for (int d = lane; d < a.cache.head_dim; d += 64) {
     float v = 0.f;
     for (int s = 0; s < a.nsplit; ++s) v += p[s * (int64_t)(dp + 2) + d] * __builtin_amdgcn_exp2f(p[s * (int64_t)(dp + 2) + dp] - ref);
-    o[d] = ElemOf<E>::put(v * inv);
+    if (a.fm != nullptr) a.fm[fm16((int)row, h * a.cache.head_dim + d, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(v * inv);
+    else o[d] = ElemOf<E>::put(v * inv);
   }
   if (lane == 0 && a.lse != nullptr) a.lse[row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
 }

@@ -226,11 +226,18 @@ int32_t msh_set_keep_encoder_output(msh_engine* e, int32_t keep) {
 
 int32_t msh_set_kv_dtype(msh_engine* e, int32_t dtype) {
   return guarded(e, [&] {
-    if (dtype != 0 && dtype != 1) throw std::invalid_argument("kv dtype: 0 = bf16, 1 = fp8 (e4m3)");
     if (e->pipe) throw std::invalid_argument("msh_set_kv_dtype: set it before msh_set_batches_in_flight (lanes take it at creation)");
-    e->eng->set_kv_fp8(dtype == 1);
+    e->eng->set_kv_dtype(dtype);
   });
 }
+
+int32_t msh_set_beam_width(msh_engine* e, int32_t width, float length_penalty) {
+  return guarded(e, [&] {
+    if (e->pipe) throw std::invalid_argument("msh_set_beam_width: set it before msh_set_batches_in_flight (lanes take it at creation)");
+    e->eng->set_beam_width(width, length_penalty);
+  });
+}
+int32_t msh_beam_width(const msh_engine* e) { return e != nullptr ? e->eng->beam_width() : MSH_ERR_INVALID_ARGUMENT; }
 
 int32_t msh_set_cross_mode(msh_engine* e, int32_t mode) {
   return guarded(e, [&] {

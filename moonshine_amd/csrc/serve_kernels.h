@@ -60,6 +60,8 @@ struct Kv4Attention {
   int32_t heads, batch, width, max_q, causal, window, nsplit;
   int32_t tiles;              // set by the launcher
   float scale_log2;           // softmax scale * log2(e)
+  uint16_t* fm;               // not null: the engine's decode path takes the output as bf16, fragment-major [rows16][heads * head_dim]
+                              // (kernels.h fm16), instead of `out`
 };
 // number of key ranges a launch is split into, and the floats of workspace that takes
 int kv4_attention_splits(const Kv4Attention& a, Elem type);
@@ -90,5 +92,18 @@ struct BeamState {
 constexpr int kBeamStates = 4;
 void beam_reorder(const BeamState* states, int n_states, int batch, int beams, const int32_t* parents, const int32_t* lengths,
                   int length_stride, hipStream_t s);
+
+// The decode loop around them (Engine::decode_beams).  Row r = clip * beams + beam.  tokens [rows][stride], its [0] = BOS; a beam that had
+// ended holds -1 from there on.  pos[0] = steps done, pos[1] = clips still decoding, pos[2] = steps done + 1 (rows of the caches).
+struct BeamLoop {
+  int32_t *tokens, *pos;
+  float *scores, *next_scores;
+  uint8_t *finished, *next_finished;
+  const int32_t *parents, *picked;
+  int32_t stride, beams, clips;
+};
+void beam_begin(const BeamLoop& l, int bos, const float* embed, int D, float* H, hipStream_t s);
+// after the selection and the reordering: append, end what is over its budget (max_len of the row's clip), embed the next inputs
+void beam_advance(const BeamLoop& l, const ClipMeta* row_clips, const float* embed, int D, float* H, hipStream_t s);
 
 }  // namespace msh

@@ -520,10 +520,16 @@ Transcriber::Transcriber(const TranscriberOptions& options) : opt_(options) {
   model_->batches_in_flight = opt_.batches_in_flight;
   model_->word_timestamps = opt_.word_timestamps;
   if (opt_.kv_dtype != 0) {
-    if (opt_.word_timestamps) throw std::runtime_error("kv_dtype=fp8 cannot be combined with word_timestamps (the capture reads bf16 keys)");
+    if (opt_.word_timestamps) throw std::runtime_error("kv_dtype=fp8 / mxfp4 cannot be combined with word_timestamps (the capture reads bf16 keys)");
     for (MoonshineModel::DeviceShard& d : model_->devices)
       if (msh_set_kv_dtype(d.engine, opt_.kv_dtype) != MSH_OK)
         throw std::runtime_error(std::string("kv_dtype: ") + msh_last_error(d.engine));
+  }
+  if (opt_.beam_width != 1) {
+    if (opt_.word_timestamps) throw std::runtime_error("beam_width > 1 cannot be combined with word_timestamps (the capture follows a greedy decode)");
+    for (MoonshineModel::DeviceShard& d : model_->devices)
+      if (msh_set_beam_width(d.engine, opt_.beam_width, opt_.length_penalty) != MSH_OK)
+        throw std::runtime_error(std::string("beam_width: ") + msh_last_error(d.engine));
   }
   if (opt_.model_source == TranscriberOptions::FILES) {
     if (opt_.model_path.empty()) throw std::runtime_error("Model path is null");
@@ -571,7 +577,7 @@ Transcriber::Transcriber(const TranscriberOptions& options) : opt_(options) {
     int mode = opt_.cross_attention;
     const bool needs_keys = opt_.word_timestamps || opt_.kv_dtype != 0;
     if (mode == 2 && needs_keys)
-      throw std::runtime_error("cross_attention=absorbed cannot be combined with word_timestamps or kv_dtype=fp8 (both read projected keys)");
+      throw std::runtime_error("cross_attention=absorbed cannot be combined with word_timestamps or kv_dtype=fp8 / mxfp4 (they read projected keys)");
     for (MoonshineModel::DeviceShard& d : model_->devices) {
       int m = mode;
       if (m == 0) m = (opt_.batch_clips_given && opt_.batch_clips >= 192 && !needs_keys && msh_cross_absorbed_supported(d.engine) == 1) ? 2 : 1;
@@ -597,6 +603,7 @@ Transcriber::Transcriber(const TranscriberOptions& options) : opt_(options) {
 // (the reference's holds frontend / encoder / adapter / cross_kv / decoder_kv .ort graphs next to the same
 // json and tokenizer, core/moonshine-streaming-model.cpp:233-300).
 void Transcriber::load_streaming_model() {
+  if (opt_.beam_width != 1) throw std::runtime_error("beam_width: the streaming architectures decode greedily (their drafts are verified against it)");
   // (word_timestamps: the reference swaps in decoder_kv_with_attention.ort here, core/transcriber.cpp:327-345; this engine
   //  computes the attention of the final token sequence on request, StreamingEngine::cross_attention)
   const int frames = (int)ceilf(opt_.max_stream_seconds * 50.0f);

@@ -67,6 +67,8 @@ def load_library(path: str | None = None) -> C.CDLL:
         "msh_set_keep_encoder_output": (i32, [vp, i32]),
         "msh_get_encoder_output": (i32, [vp, u32, vp]),
         "msh_set_kv_dtype": (i32, [vp, i32]),
+        "msh_set_beam_width": (i32, [vp, i32, f32]),
+        "msh_beam_width": (i32, [vp]),
         "msh_set_cross_mode": (i32, [vp, i32]),
         "msh_set_uniform_kernels": (i32, [vp, i32]),
         "msh_uniform_kernels": (i32, [vp]),
@@ -188,7 +190,7 @@ DECLARED_SYMBOLS = [
     "msh_stream_profile_enable", "msh_stream_profile_reset", "msh_stream_profile_count", "msh_stream_profile_get",
     "msh_set_cross_mode", "msh_set_uniform_kernels", "msh_uniform_kernels", "msh_cross_absorbed", "msh_cross_absorbed_supported",
     "msh_stream_get_features",
-    "msh_op_last_error", "msh_page_plan", "msh_kv4_page_bytes", "msh_kv4_write", "msh_kv4_read", "msh_kv4_attention_workspace",
+    "msh_set_beam_width", "msh_beam_width", "msh_op_last_error", "msh_page_plan", "msh_kv4_page_bytes", "msh_kv4_write", "msh_kv4_read", "msh_kv4_attention_workspace",
     "msh_kv4_attention", "msh_beam_select_workspace", "msh_beam_select", "msh_beam_reorder",
 ]
 
@@ -265,8 +267,14 @@ class Engine:
         self._check(self.lib.msh_set_keep_encoder_output(self.h, 1 if keep else 0))
 
     def set_kv_dtype(self, dtype: str = "bf16"):
-        """Cross K / V storage: "bf16" (default) or "fp8" (e4m3, per-row scales fixed at load); before set_batches_in_flight."""
-        self._check(self.lib.msh_set_kv_dtype(self.h, {"bf16": 0, "fp8": 1}[dtype]))
+        """Cross K / V storage: "bf16" (default), "fp8" (e4m3, per-row scales fixed at load) or "mxfp4" (the paged 4-bit cache of
+        moonshine_amd.ops); before set_batches_in_flight."""
+        self._check(self.lib.msh_set_kv_dtype(self.h, {"bf16": 0, "fp8": 1, "mxfp4": 2}[dtype]))
+
+    def set_beam_width(self, width: int = 1, length_penalty: float = 1.0):
+        """Hypotheses per clip (1 = greedy); the best accumulated log probability / ids ** length_penalty is returned; before
+        set_batches_in_flight."""
+        self._check(self.lib.msh_set_beam_width(self.h, width, length_penalty))
 
     def set_cross_mode(self, mode: str = "kv"):
         """Form of the decoder's cross-attention, ONE per engine whatever the batch size: "kv" (projected K^T / V^T stream,
