@@ -355,7 +355,7 @@ MSH_EXPORT int64_t msh_kv4_page_bytes(int32_t heads, int32_t page_size, int32_t 
  * keeps its entries for the tokens held before, gets pages from free_pages (in order: request by request) for the others, and -1 behind
  * them.  slots [rows] receives every row's slot, -1 for rows of no request.  used[0] = pages taken from free_pages; if it exceeds
  * n_free, the entries that found no page and the slots in them are -1.  Lengths are cut to [0, table_width * page_size], new_lens to
- * [0, kv_lens].  The rows of two requests must not overlap and row_start must not decrease. */
+ * [0, kv_lens].  The rows of two requests must not overlap and row_start must not decrease (a slot before such a step is not written). */
 MSH_EXPORT int32_t msh_page_plan(int32_t device, void* stream, int32_t* block_table, int32_t batch, int32_t table_width,
                                  const int32_t* kv_lens, const int32_t* new_lens, const int32_t* row_start, int64_t rows,
                                  const int32_t* free_pages, int64_t n_free, int32_t page_size, int64_t* slots, int32_t* used);

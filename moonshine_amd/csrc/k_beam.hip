@@ -15,10 +15,12 @@ __device__ __forceinline__ void wave_fence() {   // shared memory written by one
 // ---- selection ----------------------------------------------------------------------------------------------------------
 // score(k, v) = score_k + l_kv - log sum_v exp l_kv; the `beams` best of all (k, v), ties to the lowest k * vocab + v.
 // Pass 1, one wave per (row, part): running maximum and sum of exponentials, and the part's `beams` best logits in order -- the order
-//   inside a row does not depend on its sum.  Elements stay in registers (32 a lane): the K-th largest of the 64 lanes' maxima bounds
-//   the K-th largest element from below, so that all but a handful are dismissed by one comparison; later elements are held
-//   against the K-th best found so far.  One read of the logits: bound by HBM bandwidth for batches, by latency for one clip.
-// Pass 2, one workgroup per batch entry: joins the parts, ranks beams * parts * beams candidates.
+//   inside a row does not depend on its sum.  Elements stay in registers (32 a lane); the next 32 are in flight.  The K-th largest of
+//   the 64 lanes' maxima bounds the K-th largest element from below, so that all but a handful are dismissed by one comparison;
+//   later elements are held against that bound, and the list of what passed is ranked once.  One read of the logits: bound by HBM bandwidth for batches, by
+//   latency (and the fetch of its own instructions: rare paths are loops, not copies) for one clip.
+// Pass 2, one workgroup per batch entry: joins the rows' sums, takes from the parts' lists what reaches the K-th largest list head,
+//   ranks those few by counting.
 // The sums are added in 64 bits from 32 exponentials at a time and the scores compared in 64 bits: the order of two candidates of
 // different beams hangs on both rows' sums.
 struct Part {
@@ -32,10 +34,58 @@ struct Entry {
 };
 __host__ __device__ inline size_t part_bytes(int beams) { return sizeof(Part) + sizeof(Entry) * beams; }
 
-constexpr int kLane = 32;                               // elements of a lane per chunk
-constexpr int kListMax = kBeamMax * kLane + 2 * kBeamMax;   // elements above the bound lie in at most K lanes; K earlier ones, K ties
+constexpr int kLane = 32;                                      // elements of a lane per chunk
+constexpr int kListMax = 2 * kBeamMax + kBeamMax * (kLane + 1);   // room for one chunk's most beside 2 K
+constexpr int kPartsMax = 64;                                  // a wave of pass 2 joins a row's parts
+constexpr int kPicks = 1024;                                   // beams * parts * beams at most
 
 __device__ __forceinline__ bool before(const Entry& a, const Entry& b) { return a.val > b.val || (a.val == b.val && a.idx < b.idx); }
+
+// reductions over the wave along the lanes' own paths (row shifts, row broadcasts): no shared memory; the result in every lane
+template <int CTRL>
+__device__ __forceinline__ float lanes_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = lanes_max<0x111>(v);   // row_shr 1, 2, 4, 8, row_bcast 15, 31
+  v = lanes_max<0x112>(v);
+  v = lanes_max<0x114>(v);
+  v = lanes_max<0x118>(v);
+  v = lanes_max<0x142>(v);
+  v = lanes_max<0x143>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// the K-th largest of the lanes' values, one lane taken away each time
+__device__ __forceinline__ float wave_kth(float v, int K, int lane) {
+  float kth = -INFINITY;
+#pragma unroll 1
+  for (int k = 0; k < K; ++k) {
+    kth = wave_max(v);
+    const uint64_t at = __builtin_amdgcn_ballot_w64(v == kth);
+    if (lane == __ffsll((unsigned long long)at) - 1) v = -INFINITY;
+  }
+  return kth;
+}
+
+// list[0 .. n) -> the K best in order, by counting; returns how many there are
+__device__ __forceinline__ int rank_list(const Entry* list, Entry* best, int n, int K, int lane) {
+  wave_fence();
+#pragma unroll 1
+  for (int i = lane; i < n; i += 64) {
+    const Entry mine = list[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += before(list[j], mine) ? 1 : 0;
+    if (rank < K) best[rank] = mine;
+  }
+  wave_fence();
+  return n < K ? n : K;
+}
 
 template <Elem E>
 __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int parts, uint8_t* work) {
@@ -44,10 +94,8 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
   __shared__ Entry list_s[4][kListMax];
   __shared__ Entry best_s[4][kBeamMax];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  const int64_t row = id / parts;
-  const int part = (int)(id % parts);
-  if (row >= (int64_t)a.batch * a.beams) return;
+  const int id = (int)blockIdx.x * 4 + wave, row = id / parts, part = id - row * parts;
+  if (row >= a.batch * a.beams) return;
   const float score = a.scores[row];
   if (a.finished[row] != 0 || !(score > -INFINITY)) return;   // its logits are not looked at
   Entry* list = list_s[wave];
@@ -64,45 +112,58 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
 
   float top = -INFINITY;    // of this lane
   double sum = 0.0;
-  int have = 0;             // entries of `best`
+  int n = 0;                // entries of the list
+  float bound = -INFINITY;  // every element that can be among the K best so far and is not in the list yet is above it
+  bool enough = false;      // K elements of the list reach the bound
+  uint4 raw[LOADS];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int i = base + l * 64 + lane;
+      raw[l] = i < v1 ? vec[i] : uint4{0, 0, 0, 0};
+    }
+  };
+  fetch(v0);
+#pragma unroll 1
   for (int base = v0; base < v1; base += 64 * LOADS) {
     float x[kLane];
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
-      const int i = base + l * 64 + lane;
-      const uint4 u = i < v1 ? vec[i] : uint4{0, 0, 0, 0};
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      if constexpr (sizeof(T) == 4) {
+      const uint32_t w[4] = {raw[l].x, raw[l].y, raw[l].z, raw[l].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[l * 4 + e] = __uint_as_float(w[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[l * 8 + 2 * e] = ElemOf<E>::get((T)w[e]), x[l * 8 + 2 * e + 1] = ElemOf<E>::get((T)(w[e] >> 16));
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) x[l * 4 + e] = __uint_as_float(w[e]);
+        else if constexpr (E == Elem::bf16) x[l * 8 + 2 * e] = __uint_as_float(w[e] << 16), x[l * 8 + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        else x[l * 8 + 2 * e] = ElemOf<E>::get((T)w[e]), x[l * 8 + 2 * e + 1] = ElemOf<E>::get((T)(w[e] >> 16));
       }
     }
-    if (base * VEC < off || (base + 64 * LOADS) * VEC > a.vocab + off || base + 64 * LOADS > v1) {
+    if (base + 64 * LOADS < v1) fetch(base + 64 * LOADS);
+    const int first = base * VEC + lane * VEC - off;   // index of this lane's element 0; element e: + (e / VEC) * 64 * VEC + e % VEC
+    if (base == 0 || base + 64 * LOADS >= v1) {        // the row's ends and the part's
 #pragma unroll
       for (int e = 0; e < kLane; ++e) {
-        const int i = base + (e / VEC) * 64 + lane, idx = i * VEC + e % VEC - off;
-        if (i >= v1 || idx < 0 || idx >= a.vocab) x[e] = -INFINITY;
+        const int idx = first + (e / VEC) * 64 * VEC + e % VEC;
+        if (base + (e / VEC) * 64 + lane >= v1 || idx < 0 || idx >= a.vocab) x[e] = -INFINITY;
       }
     }
-    float hi = -INFINITY, now, part_sum;
-    auto sums = [&] {
-      hi = -INFINITY;
+    float hi, group[4], now, part_sum;
+    while (true) {
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) hi = fmaxf(hi, x[e]);
+      for (int q = 0; q < 4; ++q) {
+        group[q] = x[8 * q];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) group[q] = fmaxf(group[q], x[8 * q + e]);
+      }
+      hi = fmaxf(fmaxf(group[0], group[1]), fmaxf(group[2], group[3]));
       now = fmaxf(top, hi);
       const float ref = now == -INFINITY ? 0.f : now;
       part_sum = 0.f;
 #pragma unroll
       for (int e = 0; e < kLane; ++e) part_sum += __builtin_amdgcn_exp2f((x[e] - ref) * 1.44269504088896341f);
-    };
-    sums();
-    if (__builtin_amdgcn_ballot_w64(!(part_sum < INFINITY)) != 0) {   // NaN counts as -inf, +inf as the largest finite value
+      if (__builtin_amdgcn_ballot_w64(!(part_sum < INFINITY)) == 0) break;
+      // NaN counts as -inf, +inf as the largest finite value
 #pragma unroll
       for (int e = 0; e < kLane; ++e) x[e] = x[e] != x[e] ? -INFINITY : fminf(x[e], FLT_MAX);
-      sums();
     }
     if (now > top) {
       sum *= top == -INFINITY ? 0.0 : (double)__builtin_amdgcn_exp2f((top - now) * 1.44269504088896341f);
@@ -110,231 +171,224 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
     }
     sum += (double)part_sum;
 
-    // bound: K entries found -> only what is better counts; otherwise the K-th largest lane maximum
-    float bound = have == K ? best[K - 1].val : -INFINITY;
-    if (__builtin_amdgcn_ballot_w64(hi > bound) == 0) continue;
-    bool strict = have == K;   // an equal value has a higher index than what was found before
-    if (__popcll(__builtin_amdgcn_ballot_w64(hi > bound)) > K) {
-      float left = hi;
-      float kth = -INFINITY;
-      for (int k = 0; k < K; ++k) {
-        kth = left;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) kth = fmaxf(kth, __shfl_xor(kth, o));
-        const uint64_t at = __builtin_amdgcn_ballot_w64(left == kth);
-        if (lane == __ffsll((unsigned long long)at) - 1) left = -INFINITY;
-      }
-      if (kth > bound) bound = kth, strict = false;
+    // what is above the bound joins the list; until K elements are known to reach it, the K-th largest lane maximum becomes the bound
+    const int over = __popcll(__builtin_amdgcn_ballot_w64(hi > bound));
+    if (over == 0) continue;
+    if (n > kListMax - K * (kLane + 1)) {   // (a chunk adds K * 32 elements and K ties at most)
+      n = rank_list(list, best, n, K, lane);
+      if (lane < n) list[lane] = best[lane];
+      if (n == K) bound = fmaxf(bound, best[K - 1].val), enough = true;
+      wave_fence();
     }
-    int n = 0;
-    for (int k = lane; k < have; k += 64) list[k] = best[k];
-    n = have;
-    if (__builtin_amdgcn_ballot_w64(hi > bound) != 0) {
+    const bool raise = over > K && !enough;
+    if (raise) bound = wave_kth(hi, K, lane);
+    const int n0 = n;
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) {
+    for (int q = 0; q < 4; ++q) {
+      if (__builtin_amdgcn_ballot_w64(group[q] > bound) == 0) continue;
+#pragma unroll
+      for (int e = 8 * q; e < 8 * q + 8; ++e) {
         const bool in = x[e] > bound;
         const uint64_t m = __builtin_amdgcn_ballot_w64(in);
         if (m != 0) {
-          const int at = n + __popcll(m & ((1ull << lane) - 1));
-          if (in) list[at] = Entry{x[e], (base + (e / VEC) * 64 + lane) * VEC + e % VEC - off};
+          if (in) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = Entry{x[e], first + (e / VEC) * 64 * VEC + e % VEC};
           n += __popcll(m);
         }
       }
     }
-    // equal to the bound: the lowest indices, as many as can still count
-    if (!strict && bound > -INFINITY) {
-      int next = INT_MAX;   // this lane's lowest index not taken yet
-      auto seek = [&](int after) {
-        next = INT_MAX;
+    if (raise) {   // equal to the bound: the lowest indices, as many as can still count (in later chunks an equal value comes behind them)
+      int after = -1;
+#pragma unroll 1
+      for (int k = n - n0; k < K; ++k) {
+        int next = INT_MAX;   // this lane's lowest index behind `after`
 #pragma unroll
         for (int e = kLane - 1; e >= 0; --e) {
-          const int idx = (base + (e / VEC) * 64 + lane) * VEC + e % VEC - off;
+          const int idx = first + (e / VEC) * 64 * VEC + e % VEC;
           if (x[e] == bound && idx > after) next = idx;
         }
-      };
-      seek(-1);
-      for (int k = n - have; k < K; ++k) {
         int lowest = next;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) lowest = min(lowest, __shfl_xor(lowest, o));
         if (lowest == INT_MAX) break;
-        if (next == lowest) {
-          list[n] = Entry{bound, lowest};
-          seek(lowest);
-        }
+        if (next == lowest) list[n] = Entry{bound, lowest};
+        after = lowest;
         ++n;
       }
+      enough = true;
     }
-    wave_fence();
-    // rank by counting
-    const int keep = n < K ? n : K;
-    for (int i = lane; i < n; i += 64) {
-      const Entry mine = list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += before(list[j], mine) ? 1 : 0;
-      if (rank < K) best[rank] = mine;
-    }
-    have = keep;
     wave_fence();
   }
+  const int have = rank_list(list, best, n, K, lane);
 
-  float all = top;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o));
-  double total = top == -INFINITY ? 0.0 : sum * exp((double)top - (double)all);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
-  uint8_t* out = work + (row * parts + part) * part_bytes(K);
+  const float all = wave_max(top);
+  const double total = wave_sum(top == -INFINITY ? 0.0 : sum * (double)__builtin_amdgcn_exp2f((top - all) * 1.44269504088896341f));
+  uint8_t* out = work + (int64_t)id * part_bytes(K);
   if (lane == 0) *reinterpret_cast<Part*>(out) = Part{total, all, 0};
   if (lane < K) reinterpret_cast<Entry*>(out + sizeof(Part))[lane] = lane < have ? best[lane] : Entry{-INFINITY, INT_MAX};
 }
 
-constexpr int kCandidates = 16;   // of a thread of pass 2
+struct Pick {
+  double score;
+  int flat;   // beam * vocab + id: below 2^28
+  int pad;
+};
+__device__ __forceinline__ bool before(const Pick& a, const Pick& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
 
 __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts, const uint8_t* work) {
   __shared__ double offset_s[kBeamMax];
-  __shared__ double top_s[4];
-  __shared__ int64_t flat_s[4];
-  __shared__ double picked_s[kBeamMax];
-  __shared__ int64_t picked_flat_s[kBeamMax];
-  const int K = a.beams, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row0 = (int64_t)blockIdx.x * K;
-  if (threadIdx.x < K) {   // score_k - log sum exp of row k; NaN: a finished or dead beam
-    const int64_t row = row0 + threadIdx.x;
-    double o = __builtin_nan("");
-    if (a.finished[row] == 0 && a.scores[row] > -INFINITY) {
-      float top = -INFINITY;
-      for (int p = 0; p < parts; ++p) top = fmaxf(top, reinterpret_cast<const Part*>(work + (row * parts + p) * part_bytes(K))->top);
-      double sum = 0.0;
-      for (int p = 0; p < parts; ++p) {
-        const Part* q = reinterpret_cast<const Part*>(work + (row * parts + p) * part_bytes(K));
-        if (q->top > -INFINITY) sum += q->sum * exp((double)q->top - (double)top);
-      }
-      if (top > -INFINITY) o = (double)a.scores[row] - (log(sum) + (double)top);
+  __shared__ float bound_s[4];
+  __shared__ Pick list_s[kPicks];
+  __shared__ int n_s;
+  const int K = a.beams, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row0 = (int)blockIdx.x * K, stride = (int)part_bytes(K);
+  work += (int64_t)row0 * parts * stride;
+  if (threadIdx.x == 0) n_s = 0;
+  // score_k - log sum exp of row k, a wave each; -inf: a beam with no candidates of its own (finished, not in use)
+  for (int k = wave; k < K; k += 4) {
+    const float score = a.scores[row0 + k];
+    double o = -INFINITY;
+    if (a.finished[row0 + k] == 0 && score > -INFINITY) {
+      Part q{0.0, -INFINITY, 0};
+      if (lane < parts) q = *reinterpret_cast<const Part*>(work + (k * parts + lane) * stride);
+      const float top = wave_max(q.top);
+      // (the differences of the parts' maxima in 64 bits: far below 32 bits' rounding of the exponent)
+      const double sum = wave_sum(q.top == -INFINITY ? 0.0 : q.sum * exp((double)q.top - (double)top));
+      if (top > -INFINITY) o = (double)score - (log(sum) + (double)top);
     }
-    offset_s[threadIdx.x] = o;
+    if (lane == 0) offset_s[k] = o;
   }
   __syncthreads();
-  double val[kCandidates];
-  int64_t flat[kCandidates];
-  const int total = K * parts * K;
-#pragma unroll
-  for (int c = 0; c < kCandidates; ++c) {
-    val[c] = -INFINITY, flat[c] = INT64_MAX;
-    const int i = c * 256 + (int)threadIdx.x;
-    if (i >= total) continue;
-    const int k = i / (parts * K), p = i / K % parts, e = i % K;
-    const int64_t row = row0 + k;
-    if (a.finished[row] != 0) {
-      if (p == 0 && e == 0 && a.scores[row] > -INFINITY) val[c] = a.scores[row], flat[c] = (int64_t)k * a.vocab + (a.eos > 0 ? a.eos : 0);
-      continue;
+  // a thread holds one list (beam, part), best first; a finished beam's first list is the beam itself
+  const int k = (int)threadIdx.x / parts, p = (int)threadIdx.x - k * parts;
+  double offset = -INFINITY;
+  const Entry* entries = nullptr;
+  int flat0 = k * a.vocab, self = -1;
+  double head = -INFINITY;
+  if (k < K) {
+    offset = offset_s[k];
+    if (a.finished[row0 + k] != 0) {
+      if (p == 0) self = flat0 + (a.eos > 0 ? a.eos : 0), head = (double)a.scores[row0 + k];
+    } else if (offset > -INFINITY) {
+      entries = reinterpret_cast<const Entry*>(work + (k * parts + p) * stride + sizeof(Part));
+      head = offset + (double)entries[0].val;
     }
-    const double o = offset_s[k];
-    if (!(o == o)) continue;
-    const Entry en = reinterpret_cast<const Entry*>(work + (row * parts + p) * part_bytes(K) + sizeof(Part))[e];
-    if (en.val > -INFINITY) val[c] = o + (double)en.val, flat[c] = (int64_t)k * a.vocab + en.idx;
   }
-  for (int k = 0; k < K; ++k) {
-    double v = -INFINITY;
-    int64_t f = INT64_MAX;
-#pragma unroll
-    for (int c = 0; c < kCandidates; ++c)
-      if (val[c] > v || (val[c] == v && flat[c] < f)) v = val[c], f = flat[c];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const double v2 = __shfl_xor(v, o);
-      const int64_t f2 = __shfl_xor(f, o);
-      if (v2 > v || (v2 == v && f2 < f)) v = v2, f = f2;
+  const float kth = wave_kth((float)head, K, lane);
+  if (lane == 0) bound_s[wave] = kth;
+  __syncthreads();
+  const float bound = fmaxf(fmaxf(bound_s[0], bound_s[1]), fmaxf(bound_s[2], bound_s[3]));
+  auto add = [&](double score, int flat) { list_s[atomicAdd(&n_s, 1)] = Pick{score, flat, 0}; };   // (any order: it is ranked below)
+  if (self >= 0) {
+    if (head > -INFINITY && (float)head >= bound) add(head, self);
+  } else if (entries != nullptr) {
+#pragma unroll 1
+    for (int e = 0; e < K; ++e) {
+      const Entry en = entries[e];
+      const double v = offset + (double)en.val;
+      if (!(en.val > -INFINITY) || (float)v < bound) break;
+      add(v, flat0 + en.idx);
     }
-    if (lane == 0) top_s[wave] = v, flat_s[wave] = f;
-    __syncthreads();
-    v = top_s[0], f = flat_s[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w)
-      if (top_s[w] > v || (top_s[w] == v && flat_s[w] < f)) v = top_s[w], f = flat_s[w];
-#pragma unroll
-    for (int c = 0; c < kCandidates; ++c)
-      if (flat[c] == f) val[c] = -INFINITY, flat[c] = INT64_MAX;
-    if (threadIdx.x == 0) picked_s[k] = v, picked_flat_s[k] = f;
-    __syncthreads();
   }
-  if (threadIdx.x < K) {
-    const int k = threadIdx.x;
-    const int64_t row = row0 + k, f = picked_flat_s[k];
-    const bool empty = f == INT64_MAX;
-    const int parent = empty ? k : (int)(f / a.vocab), token = empty || a.finished[row0 + parent] != 0 ? a.eos : (int)(f % a.vocab);
-    const uint8_t done = empty || a.finished[row0 + parent] != 0 || token == a.eos;
-    a.out_scores[row] = (float)picked_s[k];
-    a.parents[row] = parent;
-    a.tokens[row] = token;
-    a.out_finished[row] = done;
+  __syncthreads();
+  const int n = n_s;
+  auto put = [&](int slot, double score, int parent, int token, bool done) {
+    a.out_scores[row0 + slot] = (float)score;
+    a.parents[row0 + slot] = parent;
+    a.tokens[row0 + slot] = token;
+    a.out_finished[row0 + slot] = done ? 1 : 0;
+  };
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const Pick mine = list_s[i];
+    int rank = 0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) rank += before(list_s[j], mine) ? 1 : 0;
+    if (rank < K) {
+      const int parent = mine.flat / a.vocab;
+      const bool over = a.finished[row0 + parent] != 0;
+      const int token = over ? a.eos : mine.flat - parent * a.vocab;
+      put(rank, mine.score, parent, token, over || token == a.eos);
+    }
   }
+  if ((int)threadIdx.x >= n && (int)threadIdx.x < K) put(threadIdx.x, -INFINITY, threadIdx.x, a.eos, true);   // too few candidates
 }
 
+// parts of a row: enough waves to fill the chip, at least a chunk each, and lists that pass 2 holds at one a thread
 int beam_parts(int batch, int beams, int vocab) {
   const int64_t rows = (int64_t)batch * beams;
-  int64_t n = (8192 + rows - 1) / rows;                         // waves that fill the chip
+  int64_t n = (8192 + rows - 1) / rows;
   const int64_t chunks = (vocab + 64 * kLane - 1) / (64 * kLane);
   n = n < chunks ? n : chunks;
-  const int64_t most = 256 * kCandidates / ((int64_t)beams * beams);
+  const int64_t most = kPicks / (beams * beams);
   n = n < most ? n : most;
+  n = n < 256 / beams ? n : 256 / beams;
+  n = n < kPartsMax ? n : kPartsMax;
   return (int)(n < 1 ? 1 : n);
 }
 
 // ---- reordering ---------------------------------------------------------------------------------------------------------
 // state[b, k, :len_b] <- state[b, parent[b, k], :len_b] in place.  A thread owns one piece (16 bytes) of all beams of (outer, b, inner): it
 // loads what its beams' parents have there, then stores -- no thread reads what another writes, whatever the parents are, and a beam
-// that continues itself is neither read nor written.  Bound by HBM bandwidth.
+// that continues itself is neither read nor written.  One piece a thread: several in turn
+// measured slower (four: 758 us instead of the figure below), since a workgroup's time is the latency of its chain of loads.  Bound by HBM
+// bandwidth.
 struct BeamStates {
   BeamState s[kBeamStates];
-  int64_t first[kBeamStates + 1];   // first workgroup of each state
-  int32_t blocks[kBeamStates];      // workgroups of one (outer, b, inner)
+  uint32_t first[kBeamStates];      // first workgroup of each state
+  uint32_t blocks[kBeamStates];     // workgroups of one (outer, b, inner)
   int32_t unit[kBeamStates];        // bytes of a piece: 16, 4 or 1, as the state's address and strides allow
 };
 
+// from[k]: the beam to read for beam k -- for a beam that stays one that is read anyway, so that no load hangs on a condition (each would be
+// waited for where its condition ends); move: bit k = beam k is written
 template <int KMAX, class P>
-__device__ __forceinline__ void move_piece(uint8_t* p, int64_t stride, const int32_t* parents, int beams, int bytes) {
+__device__ __forceinline__ void move_piece(uint8_t* p, int64_t stride, const int32_t* from, uint32_t move) {
   P v[KMAX];
 #pragma unroll
-  for (int k = 0; k < KMAX; ++k) {
-    const int from = k < beams ? parents[k] : k;
-    if (from != k && from >= 0 && from < beams) v[k] = *reinterpret_cast<const P*>(p + from * stride);
-  }
+  for (int k = 0; k < KMAX; ++k) v[k] = *reinterpret_cast<const P*>(p + from[k] * stride);
 #pragma unroll
-  for (int k = 0; k < KMAX; ++k) {
-    const int from = k < beams ? parents[k] : k;
-    if (from == k || from < 0 || from >= beams) continue;
-    if (bytes >= (int)sizeof(P)) {
-      *reinterpret_cast<P*>(p + k * stride) = v[k];
-    } else {   // the last piece of the valid rows
-      const uint8_t* w = reinterpret_cast<const uint8_t*>(&v[k]);
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(P); ++i)
-        if (i < bytes) p[k * stride + i] = w[i];
-    }
-  }
+  for (int k = 0; k < KMAX; ++k)
+    if ((move >> k) & 1) *reinterpret_cast<P*>(p + k * stride) = v[k];
 }
 
 template <int KMAX>
-__global__ __launch_bounds__(256) void beam_reorder_kernel(BeamStates all, int n_states, int batch, int beams, const int32_t* parents,
+__global__ __launch_bounds__(256) void beam_reorder_kernel(BeamStates all, int n_states, uint32_t batch, int beams, const int32_t* parents,
                                                            const int32_t* lengths, int length_stride) {
-  const int64_t block = blockIdx.x;
-  int which = 0;
-  while (which + 1 < n_states && block >= all.first[which + 1]) ++which;
-  const BeamState& s = all.s[which];
-  const int64_t at = block - all.first[which], seg = at / all.blocks[which];
-  const int64_t inner = seg % s.inner, b = seg / s.inner % batch, outer = seg / s.inner / batch;
-  int64_t rows = lengths != nullptr ? lengths[b * length_stride] : s.n_rows;
+  BeamState s = all.s[0];
+  uint32_t first = 0, blocks = all.blocks[0];
+  int unit = all.unit[0];
+#pragma unroll
+  for (int i = 1; i < kBeamStates; ++i)
+    if (i < n_states && blockIdx.x >= all.first[i]) s = all.s[i], first = all.first[i], blocks = all.blocks[i], unit = all.unit[i];
+  const uint32_t at = blockIdx.x - first, seg = at / blocks, slice = at - seg * blocks;
+  const uint32_t n_inner = (uint32_t)s.inner, rest = seg / n_inner, inner = seg - rest * n_inner, outer = rest / batch, b = rest - outer * batch;
+  const int32_t* par = parents + (int64_t)b * beams;
+  const int32_t given = *(lengths != nullptr ? lengths + (int64_t)b * length_stride : par);
+  int32_t f[KMAX], from[KMAX];
+#pragma unroll
+  for (int k = 0; k < KMAX; ++k) f[k] = par[k < beams ? k : beams - 1];
+  int64_t rows = lengths != nullptr ? given : s.n_rows;
   rows = rows < 0 ? 0 : rows > s.n_rows ? s.n_rows : rows;
   const int64_t bytes = rows * s.row_bytes;
-  uint8_t* p = static_cast<uint8_t*>(s.data) + outer * s.outer_stride + b * beams * s.beam_stride + inner * s.inner_stride;
-  const int32_t* par = parents + b * beams;
-  const int64_t piece = (at % all.blocks[which]) * 256 + threadIdx.x;
-  const int64_t o = piece * all.unit[which];
-  if (o >= bytes) return;
-  if (all.unit[which] == 16) move_piece<KMAX, uint4>(p + o, s.beam_stride, par, beams, (int)(bytes - o < 16 ? bytes - o : 16));
-  else if (all.unit[which] == 4) move_piece<KMAX, uint32_t>(p + o, s.beam_stride, par, beams, (int)(bytes - o < 4 ? bytes - o : 4));
-  else move_piece<KMAX, uint8_t>(p + o, s.beam_stride, par, beams, 1);
+  const int64_t o = (int64_t)slice * 256 * unit + (int64_t)threadIdx.x * unit;
+  uint32_t move = 0;
+  int32_t some = 0;
+#pragma unroll
+  for (int k = 0; k < KMAX; ++k)
+    if (k < beams && f[k] != k && f[k] >= 0 && f[k] < beams) move |= 1u << k, some = f[k];
+  if (move == 0 || o >= bytes) return;
+#pragma unroll
+  for (int k = 0; k < KMAX; ++k) from[k] = (move >> k) & 1 ? f[k] : some;
+  uint8_t* p = static_cast<uint8_t*>(s.data) + outer * s.outer_stride + b * (beams * s.beam_stride) + inner * s.inner_stride;
+  const int64_t stride = s.beam_stride;
+  if (o + unit <= bytes && unit == 16) {
+    move_piece<KMAX, uint4>(p + o, stride, from, move);
+  } else if (o + unit <= bytes && unit == 4) {
+    move_piece<KMAX, uint32_t>(p + o, stride, from, move);
+  } else {   // single bytes, and the last piece of the valid rows
+#pragma unroll 1
+    for (int64_t c = o; c < o + unit && c < bytes; ++c) move_piece<KMAX, uint8_t>(p + c, stride, from, move);
+  }
 }
 
 // ---- the decode loop ----------------------------------------------------------------------------------------------------
@@ -415,22 +469,23 @@ void beam_reorder(const BeamState* states, int n_states, int batch, int beams, c
     const BeamState& st = states[i];
     const int64_t bytes = st.n_rows * st.row_bytes;
     if (bytes == 0 || st.outer == 0 || st.inner == 0) continue;
-    all.s[n] = st;
-    all.first[n] = blocks;
     auto fits = [&](int64_t u) {
       return (uintptr_t)st.data % u == 0 && (st.outer == 1 || st.outer_stride % u == 0) && st.beam_stride % u == 0 &&
              (st.inner == 1 || st.inner_stride % u == 0);
     };
-    all.unit[n] = fits(16) ? 16 : fits(4) ? 4 : 1;
-    all.blocks[n] = (int32_t)((bytes + 256 * all.unit[n] - 1) / (256 * all.unit[n]));
+    const int64_t unit = fits(16) ? 16 : fits(4) ? 4 : 1, slice = 256 * unit;
+    all.s[n] = st;
+    all.first[n] = (uint32_t)blocks;
+    all.unit[n] = (int32_t)unit;
+    all.blocks[n] = (uint32_t)((bytes + slice - 1) / slice);
     blocks += st.outer * batch * st.inner * all.blocks[n];
     ++n;
   }
   if (n == 0 || beams < 2) return;
-  all.first[n] = blocks;
-  if (beams <= 4) MSH_LAUNCH(beam_reorder_kernel<4>, dim3((unsigned)blocks), dim3(256), 0, s, all, n, batch, beams, parents, lengths, length_stride);
-  else if (beams <= 8) MSH_LAUNCH(beam_reorder_kernel<8>, dim3((unsigned)blocks), dim3(256), 0, s, all, n, batch, beams, parents, lengths, length_stride);
-  else MSH_LAUNCH(beam_reorder_kernel<16>, dim3((unsigned)blocks), dim3(256), 0, s, all, n, batch, beams, parents, lengths, length_stride);
+  const dim3 grid((unsigned)blocks);
+  if (beams <= 4) MSH_LAUNCH(beam_reorder_kernel<4>, grid, dim3(256), 0, s, all, n, (uint32_t)batch, beams, parents, lengths, length_stride);
+  else if (beams <= 8) MSH_LAUNCH(beam_reorder_kernel<8>, grid, dim3(256), 0, s, all, n, (uint32_t)batch, beams, parents, lengths, length_stride);
+  else MSH_LAUNCH(beam_reorder_kernel<16>, grid, dim3(256), 0, s, all, n, (uint32_t)batch, beams, parents, lengths, length_stride);
 }
 
 }  // namespace msh

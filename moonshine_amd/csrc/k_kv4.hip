@@ -7,67 +7,63 @@ namespace {
 // ---- plan ---------------------------------------------------------------------------------------------------------------
 // need_b = ceil(len_b / P), kept_b = ceil((len_b - new_b) / P), first_b = sum of need - kept over the requests before b; table entry
 // kept_b + i of request b becomes free[first_b + i], and the row at place p of request b the slot table[b][p / P] * P + p mod P.
-// A few bytes per request: bound by the latency of its two launches.
+// One launch, one workgroup per request: each adds up the lengths of the requests before it for itself (8 bytes each, out of L2) instead of
+// waiting for a scan of its own launch, and clears the rows between its own and the next request's.  A few bytes per request: bound by
+// launch and memory latency.
 struct Plan {
   int32_t* table;
   const int32_t *kv_lens, *new_lens, *row_start, *free_pages;
   int64_t* slots;
-  int32_t *used, *first;
+  int32_t* used;
   int64_t rows, n_free;
   int32_t batch, width, page_shift;
 };
 
-__device__ __forceinline__ void plan_lens(const Plan& p, int b, int64_t& held, int64_t& fresh) {
-  const int64_t most = (int64_t)p.width << p.page_shift;
+__device__ __forceinline__ void plan_lens(const Plan& p, int b, int& held, int& fresh) {
+  const int most = p.width << p.page_shift;   // (at most 2^30)
   held = p.kv_lens[b], fresh = p.new_lens[b];
   held = held < 0 ? 0 : held > most ? most : held;
   fresh = fresh < 0 ? 0 : fresh > held ? held : fresh;
 }
-__device__ __forceinline__ int pages_of(int64_t tokens, int shift) { return (int)((tokens + (1 << shift) - 1) >> shift); }
+__device__ __forceinline__ int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
 
-// pages taken by the requests before `b`, summed by the whole workgroup (256 threads; every request's lengths are 8 bytes)
-__device__ int64_t plan_before(const Plan& p, int b, int64_t* red) {
-  int64_t sum = 0;
-  for (int i = threadIdx.x; i < b; i += 256) {
-    int64_t held, fresh;
-    plan_lens(p, i, held, fresh);
-    sum += pages_of(held, p.page_shift) - pages_of(held - fresh, p.page_shift);
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
-}
-
-// one workgroup per request: its table row, then the slots of its rows
 __global__ __launch_bounds__(256) void page_plan_kernel(Plan p) {
   __shared__ int64_t red[4];
-  const int b = blockIdx.x;
-  const int64_t first = plan_before(p, b, red);
-  int64_t held, fresh;
+  const int b = blockIdx.x, shift = p.page_shift;
+  int held, fresh;
   plan_lens(p, b, held, fresh);
-  const int kept = pages_of(held - fresh, p.page_shift), need = pages_of(held, p.page_shift);
+  const int64_t start = p.row_start[b], next = b + 1 < p.batch ? p.row_start[b + 1] : p.rows;
+  int64_t first = 0;   // pages taken by the requests before b
+  for (int i = threadIdx.x; i < b; i += 256) {
+    int h, f;
+    plan_lens(p, i, h, f);
+    first += pages_of(h, shift) - pages_of(h - f, shift);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = first;
+  __syncthreads();
+  first = red[0] + red[1] + red[2] + red[3];
+  const int kept = pages_of(held - fresh, shift), need = pages_of(held, shift);
   if (b == p.batch - 1 && threadIdx.x == 0) *p.used = (int32_t)(first + need - kept);
   int32_t* row = p.table + (int64_t)b * p.width;
-  auto page_at = [&](int c) -> int32_t {
+  auto page_at = [&](int c) -> int32_t {   // (kept entries are read, the others written: by no other workgroup)
     if (c < kept) return row[c];
     const int64_t at = first + c - kept;
     return c < need && at < p.n_free ? p.free_pages[at] : -1;
   };
-  const int64_t start = p.row_start[b];
-  for (int64_t i = threadIdx.x; i < fresh; i += 256) {   // reads of kept entries only, which no thread of the grid writes
-    const int64_t at = start + i, place = held - fresh + i;
-    if (at < 0 || at >= p.rows) continue;
-    const int32_t page = page_at((int)(place >> p.page_shift));
-    p.slots[at] = page < 0 ? -1 : ((int64_t)page << p.page_shift) + (place & ((1 << p.page_shift) - 1));
+  const int64_t from = b == 0 ? 0 : start, to = next < p.rows ? next : p.rows;   // rows this request answers for
+  for (int64_t at = from + threadIdx.x; at < to; at += 256) {
+    int64_t slot = -1;
+    const int64_t i = at - start;
+    if (i >= 0 && i < fresh) {
+      const int place = held - fresh + (int)i;
+      const int32_t page = page_at(place >> shift);
+      if (page >= 0) slot = ((int64_t)page << shift) + (place & ((1 << shift) - 1));
+    }
+    if (at >= 0) p.slots[at] = slot;
   }
   for (int c = kept + threadIdx.x; c < p.width; c += 256) row[c] = page_at(c);
-}
-
-__global__ __launch_bounds__(256) void page_plan_clear_kernel(int64_t* slots, int64_t rows) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < rows) slots[i] = -1;
 }
 
 // ---- writing ------------------------------------------------------------------------------------------------------------
@@ -90,84 +86,145 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float scale) {
   return r;
 }
 
-// four neighbouring threads hold a group of 32 elements
+// A workgroup: 4 rows x 16 (head, group) pairs x 4 quarters, a thread 8 elements of a key and of a value; its reads of a row are contiguous
+// over the heads.  Where four neighbouring rows are the four tokens of one aligned run of slots -- every prompt -- their lanes
+// exchange the value bytes (16 neighbouring lanes hold 4 tokens x 4 quarters) and store one dword of four tokens each instead of four
+// bytes.  One (head, group) a thread: a loop over the groups measured slower (its loads wait for one another).  Bound by HBM
+// bandwidth; single tokens by latency.
+__device__ __forceinline__ uint32_t lanes_rotate4(uint32_t x) {   // from the lane 4 below within the 16, cyclically
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x124 /* row_ror:4 */, 0xf, 0xf, false);
+}
+// lane c (of four lanes 4 apart) holds bytes [i] of token c; returns bytes [token] of pair i = c
+__device__ __forceinline__ uint32_t transpose4(uint32_t x, int c) {
+  uint32_t out = ((x >> (8 * c)) & 255u) << (8 * c);
+#pragma unroll
+  for (int s = 1; s < 4; ++s) {
+    x = lanes_rotate4(x);
+    const int from = (c - s) & 3;   // the token the word came from
+    out |= ((x >> (8 * c)) & 255u) << (8 * from);
+  }
+  return out;
+}
+
+struct Item {      // of a thread
+  int64_t r, slot;
+  int h, g, quarter, tok;
+  bool live, four;   // four: this lane's four rows are the four tokens of an aligned run
+};
+__device__ __forceinline__ Item item_of(const Kv4Cache& c, const int64_t* slots, int64_t rows, int m) {
+  Item it;
+  it.quarter = threadIdx.x & 3, it.tok = (threadIdx.x >> 2) & 3;
+  const int pair = (int)blockIdx.y * 16 + (threadIdx.x >> 4);
+  it.h = pair / m, it.g = pair - it.h * m;
+  // workgroups go round the eight XCDs: each takes a contiguous eighth of the rows, so that the eight workgroups that share a block's
+  // lines share an L2 (gridDim.x is a multiple of eight)
+  const uint32_t eighth = gridDim.x >> 3;
+  it.r = (int64_t)((blockIdx.x & 7) * eighth + (blockIdx.x >> 3)) * 4 + it.tok;
+  const bool in = it.r < rows && it.h < c.heads;
+  it.slot = in ? slots[it.r] : -1;
+  it.live = it.slot >= 0 && it.slot < c.pages << c.page_shift;
+  return it;
+}
+// (kept apart: the element loads are issued before the slot is looked at)
+__device__ __forceinline__ void item_run(Item& it) {
+  const uint32_t run = it.live ? (uint32_t)(it.slot >> 2) : 0u, run_hi = it.live ? (uint32_t)(it.slot >> 34) : 0u;
+  uint32_t a = run, b = run_hi, ok = it.live && (int)(it.slot & 3) == it.tok ? 1u : 0u, all = ok;
+#pragma unroll
+  for (int s = 1; s < 4; ++s) {
+    a = lanes_rotate4(a), b = lanes_rotate4(b), ok = lanes_rotate4(ok);
+    all &= ok & (a == run && b == run_hi ? 1u : 0u);
+  }
+  // (live, the same run and each its own place: that is the same answer in all four lanes)
+  it.four = all != 0;
+}
+__device__ __forceinline__ uint8_t* item_block(const Kv4Cache& c, const Item& it, int m, int& t) {
+  const int64_t page = it.slot >> c.page_shift;
+  const int place = (int)(it.slot & ((1 << c.page_shift) - 1));
+  t = place & 31;
+  return c.data + (((page * c.heads + it.h) << (c.page_shift - 5)) + (place >> 5)) * kv4_block_bytes(m);
+}
+
 template <Elem E>
 __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Cache c, Kv4Rows k, Kv4Rows v, int64_t rows, const int64_t* slots, int vec) {
   typedef typename ElemOf<E>::T T;
   const int m = kv4_groups(c.head_dim);
-  const int per = c.heads * m * 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = id / per;
-  const int in = (int)(id % per), quarter = in & 3, g = (in >> 2) % m, h = (in >> 2) / m;
-  int64_t slot = r < rows ? slots[r] : -1;
-  if (slot >= c.pages << c.page_shift) slot = -1;
-  const int d0 = g * 32 + quarter * 8;
+  Item it = item_of(c, slots, rows, m);
+  const int g = it.g, quarter = it.quarter, d0 = g * 32 + quarter * 8;
+  const bool in = it.r < rows && it.h < c.heads;
+  const T* kp = static_cast<const T*>(k.p) + it.r * k.row + it.h * k.head;
+  const T* vp = static_cast<const T*>(v.p) + it.r * v.row + it.h * v.head;
   float x[2][8];
+  if (in && vec && d0 + 8 <= c.head_dim) {
+    load_elems<E, 8>(kp + d0, x[0]);
+    load_elems<E, 8>(vp + d0, x[1]);
+  } else {
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const Kv4Rows& src = w ? v : k;
-    const T* p = static_cast<const T*>(src.p) + r * src.row + h * src.head + d0 * src.elem;
-    if (slot >= 0 && vec && d0 + 8 <= c.head_dim) {
-      load_elems<E, 8>(p, x[w]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[w][e] = slot >= 0 && d0 + e < c.head_dim ? ElemOf<E>::get(p[e * src.elem]) : 0.f;
+    for (int e = 0; e < 8; ++e) {
+      const bool there = in && d0 + e < c.head_dim;
+      x[0][e] = there ? ElemOf<E>::get(kp[(d0 + e) * k.elem]) : 0.f;
+      x[1][e] = there ? ElemOf<E>::get(vp[(d0 + e) * v.elem]) : 0.f;
     }
   }
+  item_run(it);
   uint32_t codes[2], scale[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     float a = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[w][e] = storable(x[w][e]), a = fmaxf(a, fabsf(x[w][e]));
-    a = fmaxf(a, __shfl_xor(a, 1));
-    a = fmaxf(a, __shfl_xor(a, 2));
+    a = fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0xB1 /* quad_perm 1,0,3,2 */, 0xf, 0xf, false)));
+    a = fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0x4E /* quad_perm 2,3,0,1 */, 0xf, 0xf, false)));
     scale[w] = scale_byte(a);
     codes[w] = codes8(x[w], kv4_scale(scale[w]));
   }
-  if (slot < 0) return;
-  const int64_t page = slot >> c.page_shift;
-  const int place = (int)(slot & ((1 << c.page_shift) - 1)), t = place & 31;
-  uint8_t* b = c.data + (((page * c.heads + h) << (c.page_shift - 5)) + (place >> 5)) * kv4_block_bytes(m);
+  const uint32_t run = transpose4(codes[1], it.tok);   // (every lane takes part in the exchange)
+  if (!it.live) return;
+  int t;
+  uint8_t* b = item_block(c, it, m, t);
   *reinterpret_cast<uint32_t*>(b + kv4_key_at(t, g, quarter, m)) = codes[0];
+  if (it.four) {
+    *reinterpret_cast<uint32_t*>(b + kv4_value_at(t & ~3, g, quarter * 4 + it.tok, m)) = run;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) b[kv4_value_at(t, g, quarter * 4 + i, m)] = (uint8_t)(codes[1] >> (8 * i));
+    for (int i = 0; i < 4; ++i) b[kv4_value_at(t, g, quarter * 4 + i, m)] = (uint8_t)(codes[1] >> (8 * i));
+  }
   if (quarter == 0) b[kv4_key_scale_at(t, g, m)] = (uint8_t)scale[0];
   if (quarter == 1) b[kv4_value_scale_at(t, g, m)] = (uint8_t)scale[1];
 }
 
-// ---- reading ------------------------------------------------------------------------------------------------------------
+// ---- reading: the same way round ----------------------------------------------------------------------------------------
 template <Elem E>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache c, const int64_t* slots, int64_t rows, void* kout, void* vout, int vec) {
   typedef typename ElemOf<E>::T T;
   const int m = kv4_groups(c.head_dim);
-  const int per = c.heads * m * 4;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = id / per;
-  if (r >= rows) return;
-  const int in = (int)(id % per), quarter = in & 3, g = (in >> 2) % m, h = (in >> 2) / m;
-  const int64_t slot = slots[r];
-  const int d0 = g * 32 + quarter * 8;
-  if (d0 >= c.head_dim) return;
+  Item it = item_of(c, slots, rows, m);
+  item_run(it);
+  const int g = it.g, quarter = it.quarter, d0 = g * 32 + quarter * 8;
   uint32_t codes[2] = {0, 0}, scale[2] = {127, 127};
-  if (slot >= 0 && slot < c.pages << c.page_shift) {
-    const int64_t page = slot >> c.page_shift;
-    const int place = (int)(slot & ((1 << c.page_shift) - 1)), t = place & 31;
-    const uint8_t* b = c.data + (((page * c.heads + h) << (c.page_shift - 5)) + (place >> 5)) * kv4_block_bytes(m);
+  if (it.live) {
+    int t;
+    const uint8_t* b = item_block(c, it, m, t);
     codes[0] = *reinterpret_cast<const uint32_t*>(b + kv4_key_at(t, g, quarter, m));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) codes[1] |= (uint32_t)b[kv4_value_at(t, g, quarter * 4 + i, m)] << (8 * i);
     scale[0] = b[kv4_key_scale_at(t, g, m)];
     scale[1] = b[kv4_value_scale_at(t, g, m)];
+    if (it.four) {
+      codes[1] = *reinterpret_cast<const uint32_t*>(b + kv4_value_at(t & ~3, g, quarter * 4 + it.tok, m));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes[1] |= (uint32_t)b[kv4_value_at(t, g, quarter * 4 + i, m)] << (8 * i);
+    }
   }
+  const uint32_t run = transpose4(codes[1], it.tok);
+  if (it.four) codes[1] = run;
+  if (it.r >= rows || it.h >= c.heads || d0 >= c.head_dim) return;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     const float s = kv4_scale(scale[w]);
-    uint32_t p[4] = {kv4_pair_bf16<0>(codes[w], s), kv4_pair_bf16<1>(codes[w], s), kv4_pair_bf16<2>(codes[w], s), kv4_pair_bf16<3>(codes[w], s)};
+    const uint32_t p[4] = {kv4_pair_bf16<0>(codes[w], s), kv4_pair_bf16<1>(codes[w], s), kv4_pair_bf16<2>(codes[w], s), kv4_pair_bf16<3>(codes[w], s)};
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(p[i] << 16), x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
-    T* o = static_cast<T*>(w ? vout : kout) + (r * c.heads + h) * c.head_dim + d0;
+    T* o = static_cast<T*>(w ? vout : kout) + (it.r * c.heads + it.h) * c.head_dim + d0;
     if (vec && d0 + 8 <= c.head_dim) {
       store_elems<E, 8>(o, x);
     } else {
@@ -178,7 +235,6 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache c, const int64_t
   }
 }
 
-unsigned grid_of(int64_t threads) { return (unsigned)((threads + 255) / 256); }
 bool aligned16(const void* p, std::initializer_list<int64_t> strides, size_t size) {
   if ((uintptr_t)p % 16 != 0) return false;
   for (int64_t s : strides)
@@ -190,8 +246,7 @@ bool aligned16(const void* p, std::initializer_list<int64_t> strides, size_t siz
 
 void page_plan(int32_t* table, int batch, int width, const int32_t* kv_lens, const int32_t* new_lens, const int32_t* row_start,
                int64_t rows, const int32_t* free_pages, int64_t n_free, int page_shift, int64_t* slots, int32_t* used, hipStream_t s) {
-  Plan p{table, kv_lens, new_lens, row_start, free_pages, slots, used, nullptr, rows, n_free, batch, width, page_shift};
-  if (rows > 0) MSH_LAUNCH(page_plan_clear_kernel, dim3(grid_of(rows)), dim3(256), 0, s, slots, rows);
+  const Plan p{table, kv_lens, new_lens, row_start, free_pages, slots, used, rows, n_free, batch, width, page_shift};
   MSH_LAUNCH(page_plan_kernel, dim3(batch), dim3(256), 0, s, p);
 }
 
@@ -199,7 +254,7 @@ void kv4_write(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows& v, Elem type,
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
   const int vec = k.elem == 1 && v.elem == 1 && aligned16(k.p, {k.row, k.head}, size) && aligned16(v.p, {v.row, v.head}, size);
-  const dim3 grid(grid_of(rows * c.heads * kv4_groups(c.head_dim) * 4));
+  const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
   if (type == Elem::f32) MSH_LAUNCH((kv4_write_kernel<Elem::f32>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
   else if (type == Elem::bf16) MSH_LAUNCH((kv4_write_kernel<Elem::bf16>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
   else MSH_LAUNCH((kv4_write_kernel<Elem::f16>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
@@ -209,7 +264,7 @@ void kv4_read(const Kv4Cache& c, const int64_t* slots, int64_t rows, void* k, vo
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
   const int vec = aligned16(k, {c.head_dim}, size) && aligned16(v, {c.head_dim}, size);
-  const dim3 grid(grid_of(rows * c.heads * kv4_groups(c.head_dim) * 4));
+  const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
   if (type == Elem::f32) MSH_LAUNCH((kv4_read_kernel<Elem::f32>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
   else if (type == Elem::bf16) MSH_LAUNCH((kv4_read_kernel<Elem::bf16>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
   else MSH_LAUNCH((kv4_read_kernel<Elem::f16>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
@@ -233,7 +288,7 @@ int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit) {
-  return nsplit > 1 ? (size_t)a.rows * a.heads * nsplit * (32 * kv4_groups(a.cache.head_dim) + 2) : 0;
+  return nsplit > 1 ? (size_t)a.rows * a.heads * nsplit * (32 * kv4_groups(a.cache.head_dim) + kPartPad) : 0;
 }
 void kv4_attention(const Kv4Attention& a, Elem type, hipStream_t s) {
   if (a.rows == 0 || a.batch == 0) return;

@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
     const int tq = r / per, g = r % per;
     const bool there = r < n_rows;
     row_of[rt] = there ? q0 + tq : -1;
-    head_of[rt] = head * per + g;
+    head_of[rt] = there ? head * per + g : head * per;
     const int at = len - n_q + tq;   // place of the query's own token
     w.last[rt] = !there ? -1 : a.causal ? at : len - 1;
     if (w.last[rt] >= len) w.last[rt] = len - 1;
@@ -273,15 +273,33 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
     w.top[rt] = -INFINITY, w.sum[rt] = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * M; ++i) w.acc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const T* src = static_cast<const T*>(a.q) + (there ? row_of[rt] * a.q_row + head_of[rt] * a.q_head : 0);
+    // every load is issued whatever the lane's row and element are (clamped into the row, selected afterwards): a load behind a
+    // condition of its own waits for the one before it
+    const T* src = static_cast<const T*>(a.q) + (there ? row_of[rt] : q0) * a.q_row + head_of[rt] * a.q_head;
+    float x[M][8];
+    if (a.vec) {
+#pragma unroll
+      for (int g2 = 0; g2 < M; ++g2)
+#pragma unroll
+        for (int c = 0; c < 8; c += 4) {
+          const int d = g2 * 32 + quarter * 8 + c;
+          load_elems<E, 4>(src + (d + 4 <= a.cache.head_dim ? d : a.cache.head_dim - 4), &x[g2][c]);
+        }
+    } else {
+#pragma unroll
+      for (int g2 = 0; g2 < M; ++g2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = g2 * 32 + quarter * 8 + e;
+          x[g2][e] = ElemOf<E>::get(src[d < a.cache.head_dim ? d : a.cache.head_dim - 1]);
+        }
+    }
 #pragma unroll
     for (int g2 = 0; g2 < M; ++g2) {
-      float x[8];
-      const int d0 = g2 * 32 + quarter * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = there && d0 + e < a.cache.head_dim ? ElemOf<E>::get(src[d0 + e]) : 0.f;
+      for (int e = 0; e < 8; ++e) x[g2][e] = there && g2 * 32 + quarter * 8 + e < a.cache.head_dim ? x[g2][e] : 0.f;
 #pragma unroll
-      for (int t = 0; t < Walk<M, E, RT>::QT; ++t) w.q[rt][g2][t] = take_term(x, t + 1 < Walk<M, E, RT>::QT);
+      for (int t = 0; t < Walk<M, E, RT>::QT; ++t) w.q[rt][g2][t] = take_term(x[g2], t + 1 < Walk<M, E, RT>::QT);
     }
   }
 
@@ -305,29 +323,34 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
   const int32_t* table = a.table + (int64_t)b * a.width;
   const int64_t block_bytes = kv4_block_bytes(M);
   const int in_shift = page_shift - 5, in_mask = (1 << in_shift) - 1;
-  auto at = [&](int blk, int32_t page) {
-    return a.cache.data + ((((int64_t)page * heads_kv + head) << in_shift) + (blk & in_mask)) * block_bytes;
-  };
-  auto page_of = [&](int blk) -> int32_t { return blk < blk1 ? table[blk >> in_shift] : -1; };
+  // (blocks behind the last are the last again, and a page that is not in the cache is page 0, not looked at: the loads of a step are
+  // unconditional, or each would be waited for where its condition ends)
+  auto page_of = [&](int blk) -> int32_t { return table[(blk < blk1 ? blk : blk1 - 1) >> in_shift]; };
   auto good = [&](int32_t page) { return page >= 0 && page < a.cache.pages; };
+  auto at = [&](int blk, int32_t page) {
+    return a.cache.data + ((((int64_t)(good(page) ? page : 0) * heads_kv + head) << in_shift) + ((blk < blk1 ? blk : blk1 - 1) & in_mask)) * block_bytes;
+  };
   auto plain = [&](int blk) { return blk * 32 >= all_from && blk * 32 + 32 <= all_to && blk * 32 + 32 <= len; };
 
   int blk = blk0 + (ROWS ? 0 : wave);
-  BlockBytes<M> x, y;
-  int32_t px = page_of(blk), py = page_of(blk + step);
-  if (good(px)) x.load(at(blk, px), lane);
-  while (blk < blk1) {
-    const int32_t next = page_of(blk + 2 * step);
-    if (good(py)) y.load(at(blk + step, py), lane);
-    if (good(px)) w.step(x, blk * 32, len, plain(blk), a.scale_log2, quarter);
-    blk += step;
-    if (blk >= blk1) break;
-    px = next;
-    const int32_t after = page_of(blk + 2 * step);
-    if (good(px)) x.load(at(blk + step, px), lane);
-    if (good(py)) w.step(y, blk * 32, len, plain(blk), a.scale_log2, quarter);
-    blk += step;
-    py = after;
+  if (blk < blk1) {
+    BlockBytes<M> x, y;
+    int32_t px = page_of(blk), py = page_of(blk + step);
+    x.load(at(blk, px), lane);
+    while (true) {
+      const int32_t next = page_of(blk + 2 * step);
+      y.load(at(blk + step, py), lane);
+      if (good(px)) w.step(x, blk * 32, len, plain(blk), a.scale_log2, quarter);
+      blk += step;
+      if (blk >= blk1) break;
+      px = next;
+      const int32_t after = page_of(blk + 2 * step);
+      x.load(at(blk + step, px), lane);
+      if (good(py)) w.step(y, blk * 32, len, plain(blk), a.scale_log2, quarter);
+      blk += step;
+      if (blk >= blk1) break;
+      py = after;
+    }
   }
 
 #pragma unroll
@@ -338,22 +361,31 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
 
   auto finish = [&](int64_t row, int h, int d0, const float* v, float top, float sum, bool first) {   // eight elements from d0 on
     if (a.nsplit > 1) {
-      float* p = a.part + ((row * a.heads + h) * a.nsplit + split) * (DP + 2);
-      if (d0 < DP) store_elems<Elem::f32, 2>(p + d0, v), store_elems<Elem::f32, 2>(p + d0 + 2, v + 2), store_elems<Elem::f32, 2>(p + d0 + 4, v + 4), store_elems<Elem::f32, 2>(p + d0 + 6, v + 6);
+      float* p = a.part + ((row * a.heads + h) * a.nsplit + split) * (DP + kPartPad);
+      *reinterpret_cast<float4*>(p + d0) = float4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<float4*>(p + d0 + 4) = float4{v[4], v[5], v[6], v[7]};
       if (first) p[DP] = top, p[DP + 1] = sum;
       return;
     }
     const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = v[e] * inv;
     if (a.fm != nullptr) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (d0 + e < a.cache.head_dim) a.fm[fm16((int)row, h * a.cache.head_dim + d0 + e, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(v[e] * inv);
+        if (d0 + e < a.cache.head_dim) a.fm[fm16((int)row, h * a.cache.head_dim + d0 + e, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(x[e]);
       return;
     }
     T* o = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head + d0;
+    if (a.vec) {
+      if (d0 + 4 <= a.cache.head_dim) store_elems<E, 4>(o, x);
+      if (d0 + 8 <= a.cache.head_dim) store_elems<E, 4>(o + 4, x + 4);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (d0 + e < a.cache.head_dim) o[e] = ElemOf<E>::put(v[e] * inv);
+      for (int e = 0; e < 8; ++e)
+        if (d0 + e < a.cache.head_dim) o[e] = ElemOf<E>::put(x[e]);
+    }
     if (first && a.lse != nullptr) a.lse[row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
   };
 
@@ -430,17 +462,25 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   } else if (row >= (int64_t)a.batch * a.max_q) {
     return;
   }
-  const float* p = a.part + (row * a.heads + h) * a.nsplit * (int64_t)(dp + 2);
-  float top = -INFINITY;
-  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, p[s * (int64_t)(dp + 2) + dp]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) sum += p[s * (int64_t)(dp + 2) + dp + 1] * __builtin_amdgcn_exp2f(p[s * (int64_t)(dp + 2) + dp] - ref);
+  // lane s: the maximum and the sum of range s (at most 64 of them)
+  const int64_t stride = dp + kPartPad;
+  const float* p = a.part + (row * a.heads + h) * a.nsplit * stride;
+  float mine = -INFINITY, part_sum = 0.f;
+  if (lane < a.nsplit) mine = p[lane * stride + dp], part_sum = p[lane * stride + dp + 1];
+  float top = mine;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+  float sum = part_sum * f;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   T* o = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head;
-  for (int d = lane; d < a.cache.head_dim; d += 64) {
+  for (int d = lane; d < dp; d += 64) {
     float v = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) v += p[s * (int64_t)(dp + 2) + d] * __builtin_amdgcn_exp2f(p[s * (int64_t)(dp + 2) + dp] - ref);
+#pragma unroll 8
+    for (int s = 0; s < a.nsplit; ++s) v += p[s * stride + d] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
+    if (d >= a.cache.head_dim) continue;
     if (a.fm != nullptr) a.fm[fm16((int)row, h * a.cache.head_dim + d, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(v * inv);
     else o[d] = ElemOf<E>::put(v * inv);
   }
@@ -453,6 +493,10 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
   const int64_t pairs = (int64_t)a.batch * a.cache.heads;
   a.tiles = (int32_t)(rows <= 16 ? 1 : rows <= 64 ? (rows + 31) / 32 : (rows + 127) / 128);
+  const int64_t four = E == Elem::f32 ? 16 : 8;   // bytes of four elements
+  const int64_t size = four / 4;
+  auto even = [&](const void* p, int64_t row, int64_t head) { return (uintptr_t)p % four == 0 && row * size % four == 0 && head * size % four == 0; };
+  a.vec = a.cache.head_dim % 4 == 0 && even(a.q, a.q_row, a.q_head) && (a.fm != nullptr || even(a.out, a.out_row, a.out_head));
   const dim3 grid((unsigned)(pairs * a.tiles), (unsigned)a.nsplit);
   if (rows <= 16) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, false>), grid, dim3(256), 0, s, a);
   else if (rows <= 64) MSH_LAUNCH((kv4_attention_kernel<M, E, 2, false>), grid, dim3(256), 0, s, a);
