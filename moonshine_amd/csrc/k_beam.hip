@@ -316,7 +316,8 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
 // parts of a row: enough waves to fill the chip, at least a chunk each, and lists that pass 2 holds at one a thread
 int beam_parts(int batch, int beams, int vocab) {
   const int64_t rows = (int64_t)batch * beams;
-  int64_t n = (8192 + rows - 1) / rows;
+  static const char* env = getenv("BPN");
+  int64_t n = ((env ? atoi(env) : 8192) + rows - 1) / rows;
   const int64_t chunks = (vocab + 64 * kLane - 1) / (64 * kLane);
   n = n < chunks ? n : chunks;
   const int64_t most = kPicks / (beams * beams);
@@ -341,6 +342,7 @@ struct BeamStates {
 
 // from[k]: the beam to read for beam k -- for a beam that stays one that is read anyway, so that no load hangs on a condition (each would be
 // waited for where its condition ends); move: bit k = beam k is written
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));   // (an array of HIP's uint4 class ends up in scratch memory: twice the writes)
 template <int KMAX, class P>
 __device__ __forceinline__ void move_piece(uint8_t* p, int64_t stride, const int32_t* from, uint32_t move) {
   P v[KMAX];
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamStates all, int n
   uint8_t* p = static_cast<uint8_t*>(s.data) + outer * s.outer_stride + b * (beams * s.beam_stride) + inner * s.inner_stride;
   const int64_t stride = s.beam_stride;
   if (o + unit <= bytes && unit == 16) {
-    move_piece<KMAX, uint4>(p + o, stride, from, move);
+    move_piece<KMAX, u32x4>(p + o, stride, from, move);
   } else if (o + unit <= bytes && unit == 4) {
     move_piece<KMAX, uint32_t>(p + o, stride, from, move);
   } else {   // single bytes, and the last piece of the valid rows

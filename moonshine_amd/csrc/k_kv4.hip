@@ -73,8 +73,15 @@ __device__ __forceinline__ float storable(float x) {
   x = x != x ? 0.f : x;
   return fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f);
 }
-__device__ __forceinline__ uint32_t scale_byte(float amax) {
-  const int e = (int)((__float_as_uint(amax) + 0x200000u) >> 23) - 129;
+// the largest magnitude's bits, which are ordered as the magnitudes are (infinity and NaN above all)
+__device__ __forceinline__ uint32_t abs_max8(const float* x) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a = max(a, __float_as_uint(x[e]) & 0x7fffffffu);
+  return a;
+}
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+  const int e = (int)((amax_bits + 0x200000u) >> 23) - 129;
   return (uint32_t)((e < -100 ? -100 : e > 125 ? 125 : e) + 127);
 }
 __device__ __forceinline__ uint32_t codes8(const float* x, float scale) {
@@ -111,7 +118,8 @@ struct Item {      // of a thread
   int h, g, quarter, tok;
   bool live, four;   // four: this lane's four rows are the four tokens of an aligned run
 };
-__device__ __forceinline__ Item item_of(const Kv4Cache& c, const int64_t* slots, int64_t rows, int m) {
+template <int m>
+__device__ __forceinline__ Item item_of(const Kv4Cache& c, const int64_t* slots, int64_t rows) {
   Item it;
   it.quarter = threadIdx.x & 3, it.tok = (threadIdx.x >> 2) & 3;
   const int pair = (int)blockIdx.y * 16 + (threadIdx.x >> 4);
@@ -144,36 +152,47 @@ __device__ __forceinline__ uint8_t* item_block(const Kv4Cache& c, const Item& it
   return c.data + (((page * c.heads + it.h) << (c.page_shift - 5)) + (place >> 5)) * kv4_block_bytes(m);
 }
 
-template <Elem E>
+template <Elem E, int M>
 __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Cache c, Kv4Rows k, Kv4Rows v, int64_t rows, const int64_t* slots, int vec) {
   typedef typename ElemOf<E>::T T;
-  const int m = kv4_groups(c.head_dim);
-  Item it = item_of(c, slots, rows, m);
+  constexpr int m = M;   // (groups of 32: the offsets below become shifts and adds)
+  Item it = item_of<M>(c, slots, rows);
   const int g = it.g, quarter = it.quarter, d0 = g * 32 + quarter * 8;
   const bool in = it.r < rows && it.h < c.heads;
   const T* kp = static_cast<const T*>(k.p) + it.r * k.row + it.h * k.head;
   const T* vp = static_cast<const T*>(v.p) + it.r * v.row + it.h * v.head;
   float x[2][8];
-  if (in && vec && d0 + 8 <= c.head_dim) {
-    load_elems<E, 8>(kp + d0, x[0]);
-    load_elems<E, 8>(vp + d0, x[1]);
-  } else {
+  // (loads are clamped into the row and selected afterwards: none waits for another)
+  if (in && vec) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const int d = d0 + e + 4 <= c.head_dim ? d0 + e : c.head_dim - 4;
+      load_elems<E, 4>(kp + d, &x[0][e]);
+      load_elems<E, 4>(vp + d, &x[1][e]);
+    }
+  } else if (in) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool there = in && d0 + e < c.head_dim;
-      x[0][e] = there ? ElemOf<E>::get(kp[(d0 + e) * k.elem]) : 0.f;
-      x[1][e] = there ? ElemOf<E>::get(vp[(d0 + e) * v.elem]) : 0.f;
+      const int d = d0 + e < c.head_dim ? d0 + e : c.head_dim - 1;
+      x[0][e] = ElemOf<E>::get(kp[d * k.elem]);
+      x[1][e] = ElemOf<E>::get(vp[d * v.elem]);
     }
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (!in || d0 + e >= c.head_dim) x[0][e] = x[1][e] = 0.f;
   item_run(it);
   uint32_t codes[2], scale[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    float a = 0.f;
+    uint32_t a = abs_max8(x[w]);
+    if (a >= 0x7f800000u) {   // an infinity or NaN: rare
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[w][e] = storable(x[w][e]), a = fmaxf(a, fabsf(x[w][e]));
-    a = fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0xB1 /* quad_perm 1,0,3,2 */, 0xf, 0xf, false)));
-    a = fmaxf(a, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(a), 0x4E /* quad_perm 2,3,0,1 */, 0xf, 0xf, false)));
+      for (int e = 0; e < 8; ++e) x[w][e] = storable(x[w][e]);
+      a = abs_max8(x[w]);
+    }
+    a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1 /* quad_perm 1,0,3,2 */, 0xf, 0xf, false));
+    a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E /* quad_perm 2,3,0,1 */, 0xf, 0xf, false));
     scale[w] = scale_byte(a);
     codes[w] = codes8(x[w], kv4_scale(scale[w]));
   }
@@ -193,11 +212,11 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Cache c, Kv4Rows k, K
 }
 
 // ---- reading: the same way round ----------------------------------------------------------------------------------------
-template <Elem E>
+template <Elem E, int M>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache c, const int64_t* slots, int64_t rows, void* kout, void* vout, int vec) {
   typedef typename ElemOf<E>::T T;
-  const int m = kv4_groups(c.head_dim);
-  Item it = item_of(c, slots, rows, m);
+  constexpr int m = M;   // (groups of 32: the offsets below become shifts and adds)
+  Item it = item_of<M>(c, slots, rows);
   item_run(it);
   const int g = it.g, quarter = it.quarter, d0 = g * 32 + quarter * 8;
   uint32_t codes[2] = {0, 0}, scale[2] = {127, 127};
@@ -221,24 +240,45 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache c, const int64_t
   for (int w = 0; w < 2; ++w) {
     const float s = kv4_scale(scale[w]);
     const uint32_t p[4] = {kv4_pair_bf16<0>(codes[w], s), kv4_pair_bf16<1>(codes[w], s), kv4_pair_bf16<2>(codes[w], s), kv4_pair_bf16<3>(codes[w], s)};
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(p[i] << 16), x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
     T* o = static_cast<T*>(w ? vout : kout) + (it.r * c.heads + it.h) * c.head_dim + d0;
-    if (vec && d0 + 8 <= c.head_dim) {
-      store_elems<E, 8>(o, x);
+    if (vec) {   // four elements at a time: a head width is a multiple of four then
+      if constexpr (E == Elem::bf16) {
+        *reinterpret_cast<uint2*>(o) = uint2{p[0], p[1]};
+        if (d0 + 8 <= c.head_dim) *reinterpret_cast<uint2*>(o + 4) = uint2{p[2], p[3]};
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(p[i] << 16), x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+        store_elems<E, 4>(o, x);
+        if (d0 + 8 <= c.head_dim) store_elems<E, 4>(o + 4, x + 4);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (d0 + e < c.head_dim) o[e] = ElemOf<E>::put(x[e]);
+        if (d0 + e < c.head_dim) o[e] = ElemOf<E>::put(__uint_as_float(e & 1 ? p[e / 2] & 0xffff0000u : p[e / 2] << 16));
     }
   }
 }
 
-bool aligned16(const void* p, std::initializer_list<int64_t> strides, size_t size) {
-  if ((uintptr_t)p % 16 != 0) return false;
+template <class F>
+void by_groups(int m, F&& f) {
+  switch (m) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 5: return f(std::integral_constant<int, 5>{});
+    case 6: return f(std::integral_constant<int, 6>{});
+    case 7: return f(std::integral_constant<int, 7>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    default: throw std::invalid_argument("4-bit cache: head width above 256");
+  }
+}
+// whether four elements at a time may be read or written
+bool by_fours(const void* p, std::initializer_list<int64_t> strides, int head_dim, size_t size) {
+  if (head_dim % 4 != 0 || (uintptr_t)p % (4 * size) != 0) return false;
   for (int64_t s : strides)
-    if (s * (int64_t)size % 16 != 0) return false;
+    if (s % 4 != 0) return false;
   return true;
 }
 
@@ -253,21 +293,27 @@ void page_plan(int32_t* table, int batch, int width, const int32_t* kv_lens, con
 void kv4_write(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows& v, Elem type, int64_t rows, const int64_t* slots, hipStream_t s) {
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
-  const int vec = k.elem == 1 && v.elem == 1 && aligned16(k.p, {k.row, k.head}, size) && aligned16(v.p, {v.row, v.head}, size);
+  const int vec = k.elem == 1 && v.elem == 1 && by_fours(k.p, {k.row, k.head}, c.head_dim, size) && by_fours(v.p, {v.row, v.head}, c.head_dim, size);
   const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
-  if (type == Elem::f32) MSH_LAUNCH((kv4_write_kernel<Elem::f32>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
-  else if (type == Elem::bf16) MSH_LAUNCH((kv4_write_kernel<Elem::bf16>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
-  else MSH_LAUNCH((kv4_write_kernel<Elem::f16>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
+  by_groups(kv4_groups(c.head_dim), [&](auto m) {
+    constexpr int M = decltype(m)::value;
+    if (type == Elem::f32) MSH_LAUNCH((kv4_write_kernel<Elem::f32, M>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
+    else if (type == Elem::bf16) MSH_LAUNCH((kv4_write_kernel<Elem::bf16, M>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
+    else MSH_LAUNCH((kv4_write_kernel<Elem::f16, M>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
+  });
 }
 
 void kv4_read(const Kv4Cache& c, const int64_t* slots, int64_t rows, void* k, void* v, Elem type, hipStream_t s) {
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
-  const int vec = aligned16(k, {c.head_dim}, size) && aligned16(v, {c.head_dim}, size);
+  const int vec = by_fours(k, {}, c.head_dim, size) && by_fours(v, {}, c.head_dim, size);
   const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
-  if (type == Elem::f32) MSH_LAUNCH((kv4_read_kernel<Elem::f32>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
-  else if (type == Elem::bf16) MSH_LAUNCH((kv4_read_kernel<Elem::bf16>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
-  else MSH_LAUNCH((kv4_read_kernel<Elem::f16>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
+  by_groups(kv4_groups(c.head_dim), [&](auto m) {
+    constexpr int M = decltype(m)::value;
+    if (type == Elem::f32) MSH_LAUNCH((kv4_read_kernel<Elem::f32, M>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
+    else if (type == Elem::bf16) MSH_LAUNCH((kv4_read_kernel<Elem::bf16, M>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
+    else MSH_LAUNCH((kv4_read_kernel<Elem::f16, M>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
+  });
 }
 
 // ---- attention: dispatch ------------------------------------------------------------------------------------------------
@@ -275,15 +321,30 @@ void kv4_attention_f32(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_bf16(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 
+// Rows of one key / value head: up to 16 one tile, above that tiles of 32.  Waves share a tile while there are too few tiles to fill the chip
+// (1024 SIMDs) without.
+Kv4Shape kv4_attention_shape(const Kv4Attention& a) {
+  static const char* env = getenv("KV4_SHAPE");
+  const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
+  const int rt = rows <= 16 ? 1 : 2;
+  const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + 16 * rt - 1) / (16 * rt));
+  if (env && rt == 1) return Kv4Shape{1, atoi(env)};
+  if (rt == 2) return Kv4Shape{2, rows > 64 ? 1 : 4};
+  return Kv4Shape{1, units >= 4096 ? 1 : units >= 2048 ? 2 : 4};
+}
+
 // The lengths live on the device; the host knows the table's room only.  A range is a share of each sequence's own length, so a short
 // sequence in a wide table costs empty ranges and nothing else.
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
+  const Kv4Shape shape = kv4_attention_shape(a);
+  if (shape.kw != 4) return 1;
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
-  if (rows > 64) return 1;
-  const int64_t groups = (int64_t)a.batch * a.cache.heads * ((rows + 31) / 32);
+  const int64_t groups = (int64_t)a.batch * a.cache.heads * ((rows + 16 * shape.rt - 1) / (16 * shape.rt));
   const int64_t room = (int64_t)a.width << a.cache.page_shift;
-  const int64_t most = (room + 255) / 256;   // two blocks per wave at least
-  int64_t n = (2048 + groups - 1) / groups;
+  const int64_t most = room / 512;   // four blocks per wave at least: a block takes a wave about 1 us, the second launch 3
+  static const char* env = getenv("KV4_WG");
+  const int64_t want = env ? atoi(env) : 2048;
+  int64_t n = (want + groups - 1) / groups;
   n = n < most ? n : most;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }

@@ -101,7 +101,8 @@ struct BlockBytes {
   }
 };
 
-__device__ __forceinline__ Frag expand_keys(uint32_t codes, float s) {
+__device__ __forceinline__ Frag expand_keys(uint32_t codes, uint32_t scales, int byte) {   // (byte: a constant after unrolling)
+  const float s = byte == 0 ? kv4_scale_of<0>(scales) : byte == 1 ? kv4_scale_of<1>(scales) : byte == 2 ? kv4_scale_of<2>(scales) : kv4_scale_of<3>(scales);
   Frag f;
   f.u[0] = kv4_pair_bf16<0>(codes, s);
   f.u[1] = kv4_pair_bf16<1>(codes, s);
@@ -115,8 +116,8 @@ __device__ __forceinline__ void expand_values(const uint32_t* v, const uint32_t*
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const uint32_t c = v[half], s = vs[half];
-    const uint32_t t0 = kv4_pair_bf16<0>(c, kv4_scale(s & 255)), t1 = kv4_pair_bf16<1>(c, kv4_scale((s >> 8) & 255));
-    const uint32_t t2 = kv4_pair_bf16<2>(c, kv4_scale((s >> 16) & 255)), t3 = kv4_pair_bf16<3>(c, kv4_scale(s >> 24));
+    const uint32_t t0 = kv4_pair_bf16<0>(c, kv4_scale_of<0>(s)), t1 = kv4_pair_bf16<1>(c, kv4_scale_of<1>(s));
+    const uint32_t t2 = kv4_pair_bf16<2>(c, kv4_scale_of<2>(s)), t3 = kv4_pair_bf16<3>(c, kv4_scale_of<3>(s));
     even.u[2 * half] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
     odd.u[2 * half] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
     even.u[2 * half + 1] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
@@ -152,6 +153,8 @@ struct Walk {
   int last[RT];           // last visible token of this lane's row (causal), first visible
   int low[RT];
 
+  // plain: every row sees all 32 tokens (uniform).  The empty asm keeps the masks behind their branch -- they would be computed for every
+  // block otherwise --; a second copy of the step costs more registers than it saves
   __device__ __forceinline__ void step(const BlockBytes<M>& b, int t0, int len, bool plain, float scale_log2, int quarter) {
     f32x4 s[RT][2];
 #pragma unroll
@@ -160,7 +163,7 @@ struct Walk {
       for (int rt = 0; rt < RT; ++rt) s[rt][tile] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < M; ++g) {
-        const Frag k = expand_keys(b.k[tile][g], kv4_scale((b.ks[tile][g / 4] >> (8 * (g & 3))) & 255));
+        const Frag k = expand_keys(b.k[tile][g], b.ks[tile][g / 4], g & 3);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -169,6 +172,7 @@ struct Walk {
     }
     uint32_t keep[2] = {~0u, ~0u};   // bytes of the tokens that exist, of this lane's 4 + 4
     if (!plain) {
+      asm volatile("" ::: );
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         keep[half] = 0;
@@ -176,20 +180,24 @@ struct Walk {
         for (int c = 0; c < 4; ++c)
           if (t0 + half * 16 + quarter * 4 + c < len) keep[half] |= 255u << (8 * c);
       }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int t = t0 + (e >> 2) * 16 + quarter * 4 + (e & 3);
+          s[rt][e >> 2][e & 3] = t <= last[rt] && t >= low[rt] ? s[rt][e >> 2][e & 3] : -INFINITY;
+        }
     }
     Frag p[RT][PT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[8];
+      float x[8];   // q . k (times the scale's sign)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = s[rt][e >> 2][e & 3] * scale_log2;
-        if (!plain) {
-          const int t = t0 + (e >> 2) * 16 + quarter * 4 + (e & 3);
-          x[e] = t <= last[rt] && t >= low[rt] ? x[e] : -INFINITY;
-        }
+        x[e] = s[rt][e >> 2][e & 3];
       }
       float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      hi *= scale_log2;
       if (__builtin_amdgcn_ballot_w64(hi > top[rt] + 8.f) != 0) {   // (top = -inf: any finite score)
         hi = fmaxf(hi, __shfl_xor(hi, 16));
         hi = fmaxf(hi, __shfl_xor(hi, 32));
@@ -204,7 +212,7 @@ struct Walk {
       float add = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(x[e] - ref);
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], scale_log2, -ref));
         add += x[e];
       }
       sum[rt] += add;
@@ -215,6 +223,7 @@ struct Walk {
     for (int g = 0; g < M; ++g) {
       uint32_t vs[2] = {b.vs[2 * g], b.vs[2 * g + 1]};
       if (!plain) {   // a token past the end: whatever its scale byte is, 0 * finite = 0
+        asm volatile("" ::: );
 #pragma unroll
         for (int half = 0; half < 2; ++half) vs[half] = (vs[half] & keep[half]) | (0x7f7f7f7fu & ~keep[half]);
       }
@@ -231,27 +240,38 @@ struct Walk {
   }
 };
 
-// ROWS false: the four waves of a workgroup share 16 * RT rows and take the blocks of the workgroup's range in turn; their results are
-//             joined in shared memory.  For few rows (single tokens, beams, drafts), where the cache's bytes are what counts.
-// ROWS true : every wave has 16 * RT rows of its own and walks all their blocks; for chunks of prompts.
-template <int M, Elem E, int RT, bool ROWS>
-__global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
+// KW: waves that share 16 * RT rows, take the blocks of the workgroup's range in turn and join their results in shared memory; 4 / KW such
+//   units (a tile of rows of a sequence and key / value head) make a workgroup.  KW = 4 where few rows have long caches, 1 where there
+//   are rows enough -- chunks of prompts, many short sequences --: a wave's beginning and end cost as much as three blocks.
+// waves per SIMD: left alone the compiler spends the registers of two or three waves on one; asked for more it spills
+template <int M, Elem E, int RT>
+constexpr int waves_wanted() {
+  if (RT == 1) return M <= 2 ? 4 : M <= 4 && E != Elem::f32 ? 3 : 2;
+  return M <= 2 ? (E == Elem::bf16 ? 3 : 2) : M <= 4 && E != Elem::f32 ? 2 : 1;
+}
+template <int M, Elem E, int RT, int KW>
+__global__ __launch_bounds__(256, (waves_wanted<M, E, RT>())) void kv4_attention_kernel(Kv4Attention a) {
   typedef typename ElemOf<E>::T T;
   constexpr int DP = 32 * M;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int quarter = lane >> 4, idx = lane & 15;
   const int heads_kv = a.cache.heads, per = a.heads / heads_kv;
-  // workgroup = ((sequence, key / value head), tile of rows); the second grid axis is the key range
-  const int tile0 = (int)(blockIdx.x % a.tiles), pair = (int)(blockIdx.x / a.tiles), split = blockIdx.y;
-  const int head = pair % heads_kv, b = pair / heads_kv;
+  // unit = ((sequence, key / value head), tile of rows); the second grid axis is the key range
+  const int sub = wave % KW, unit = (int)blockIdx.x * (4 / KW) + wave / KW, split = blockIdx.y;
+  const int pair = unit / a.tiles, tile0 = unit - pair * a.tiles;
+  int b = pair / heads_kv;
+  const int head = pair - b * heads_kv;
+  bool active = b < a.batch;   // (a wave without work stays for the barriers of its workgroup)
+  b = active ? b : 0;
   const int page_shift = a.cache.page_shift;
   const int64_t q0 = a.q_start != nullptr ? a.q_start[b] : (int64_t)b * a.max_q;
   int n_q = a.q_start != nullptr ? a.q_start[b + 1] - a.q_start[b] : a.max_q;
   if (n_q > a.max_q) n_q = a.max_q;
-  if (q0 < 0 || n_q <= 0 || q0 + n_q > a.rows) return;   // (a q_start that does not fit: nothing is written)
-  const int n_rows = n_q * per;
-  const int row0 = (ROWS ? tile0 * 4 + wave : tile0) * 16 * RT;
-  if (row0 >= n_rows) return;                            // ROWS: a wave; otherwise the whole workgroup
+  active = active && q0 >= 0 && n_q > 0 && q0 + n_q <= a.rows;   // (a q_start that does not fit: nothing is written)
+  const int n_rows = active ? n_q * per : 0;
+  const int row0 = tile0 * 16 * RT;
+  active = active && row0 < n_rows;
+  if (KW == 1 && !active) return;
   int len = a.kv_lens[b];
   const int64_t room = (int64_t)a.width << page_shift;
   len = len < 0 ? 0 : len > room ? (int)room : len;
@@ -275,7 +295,7 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
     for (int i = 0; i < 2 * M; ++i) w.acc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     // every load is issued whatever the lane's row and element are (clamped into the row, selected afterwards): a load behind a
     // condition of its own waits for the one before it
-    const T* src = static_cast<const T*>(a.q) + (there ? row_of[rt] : q0) * a.q_row + head_of[rt] * a.q_head;
+    const T* src = static_cast<const T*>(a.q) + (there ? row_of[rt] : active ? q0 : 0) * a.q_row + head_of[rt] * a.q_head;
     float x[M][8];
     if (a.vec) {
 #pragma unroll
@@ -297,7 +317,7 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
 #pragma unroll
     for (int g2 = 0; g2 < M; ++g2) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[g2][e] = there && g2 * 32 + quarter * 8 + e < a.cache.head_dim ? x[g2][e] : 0.f;
+      for (int e = 0; e < 8; ++e) x[g2][e] = there && g2 * 32 + quarter * 8 + e < a.cache.head_dim ? x[g2][e] * a.sign : 0.f;
 #pragma unroll
       for (int t = 0; t < Walk<M, E, RT>::QT; ++t) w.q[rt][g2][t] = take_term(x[g2], t + 1 < Walk<M, E, RT>::QT);
     }
@@ -319,7 +339,7 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
     blk1 = s0 + share < blk1 ? s0 + share : blk1;
     blk0 = s0;
   }
-  const int step = ROWS ? 1 : 4;
+  if (!active) blk1 = blk0;
   const int32_t* table = a.table + (int64_t)b * a.width;
   const int64_t block_bytes = kv4_block_bytes(M);
   const int in_shift = page_shift - 5, in_mask = (1 << in_shift) - 1;
@@ -332,21 +352,23 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
   };
   auto plain = [&](int blk) { return blk * 32 >= all_from && blk * 32 + 32 <= all_to && blk * 32 + 32 <= len; };
 
-  int blk = blk0 + (ROWS ? 0 : wave);
+  constexpr int step = KW;
+  int blk = blk0 + sub;
   if (blk < blk1) {
     BlockBytes<M> x, y;
     int32_t px = page_of(blk), py = page_of(blk + step);
+    auto walk = [&](const BlockBytes<M>& bytes) { w.step(bytes, blk * 32, len, plain(blk), a.scale_log2, quarter); };
     x.load(at(blk, px), lane);
     while (true) {
       const int32_t next = page_of(blk + 2 * step);
       y.load(at(blk + step, py), lane);
-      if (good(px)) w.step(x, blk * 32, len, plain(blk), a.scale_log2, quarter);
+      if (good(px)) walk(x);
       blk += step;
       if (blk >= blk1) break;
       px = next;
       const int32_t after = page_of(blk + 2 * step);
       x.load(at(blk + step, px), lane);
-      if (good(py)) w.step(y, blk * 32, len, plain(blk), a.scale_log2, quarter);
+      if (good(py)) walk(y);
       blk += step;
       if (blk >= blk1) break;
       py = after;
@@ -389,7 +411,7 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
     if (first && a.lse != nullptr) a.lse[row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
   };
 
-  if constexpr (ROWS) {
+  if constexpr (KW == 1) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (row_of[rt] < 0) continue;
@@ -402,10 +424,10 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
       }
     }
   } else {
-    // rows of 8 floats are skewed by 4 every 32 so that the 16 rows' stores and loads spread over the banks
-    constexpr int LD = DP + 4;
+    constexpr int LD = DP + 4;   // (16 rows' 16-byte pieces spread over the banks)
     __shared__ float part[4][16][LD];
     __shared__ float stat[4][16][2];
+    const int first_wave = wave - sub;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (rt > 0) __syncthreads();
@@ -418,20 +440,20 @@ __global__ __launch_bounds__(256) void kv4_attention_kernel(Kv4Attention a) {
         *reinterpret_cast<float4*>(&part[wave][idx][g * 32 + quarter * 8 + 4]) = hi;
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < 16 * 4 * M; i += 256) {
+      for (int i = sub * 64 + lane; i < 16 * 4 * M; i += KW * 64) {
         const int col = i / (4 * M), d0 = (i % (4 * M)) * 8, r = row0 + rt * 16 + col;
         if (r >= n_rows) continue;
-        float top = stat[0][col][0];
+        float top = stat[first_wave][col][0];
 #pragma unroll
-        for (int v = 1; v < 4; ++v) top = fmaxf(top, stat[v][col][0]);
+        for (int v = 1; v < KW; ++v) top = fmaxf(top, stat[first_wave + v][col][0]);
         const float ref = top == -INFINITY ? 0.f : top;
         float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float f = __builtin_amdgcn_exp2f(stat[v][col][0] - ref);
-          sum += stat[v][col][1] * f;
+        for (int v = 0; v < KW; ++v) {
+          const float f = __builtin_amdgcn_exp2f(stat[first_wave + v][col][0] - ref);
+          sum += stat[first_wave + v][col][1] * f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] += part[v][col][d0 + e] * f;
+          for (int e = 0; e < 8; ++e) o[e] += part[first_wave + v][col][d0 + e] * f;
         }
         finish(q0 + r / per, head * per + r % per, d0, o, top, sum, d0 == 0);
       }
@@ -476,13 +498,30 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   T* o = static_cast<T*>(a.out) + row * a.out_row + h * a.out_head;
-  for (int d = lane; d < dp; d += 64) {
-    float v = 0.f;
+  // a lane has four elements; where those take up half the wave or less, groups of lanes take the ranges in turn: all rows are in flight at once
+  const int per = dp >> 2, groups = 64 / per, group = lane / per, d0 = (lane - group * per) * 4;
+  float4 v{0.f, 0.f, 0.f, 0.f};
+  if (group < groups) {
 #pragma unroll 8
-    for (int s = 0; s < a.nsplit; ++s) v += p[s * stride + d] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-    if (d >= a.cache.head_dim) continue;
-    if (a.fm != nullptr) a.fm[fm16((int)row, h * a.cache.head_dim + d, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(v * inv);
-    else o[d] = ElemOf<E>::put(v * inv);
+    for (int s = group; s < a.nsplit; s += groups) {
+      const float4 x = *reinterpret_cast<const float4*>(p + s * stride + d0);
+      const float g = __shfl(f, s);
+      v.x += x.x * g, v.y += x.y * g, v.z += x.z * g, v.w += x.w * g;
+    }
+  }
+  for (int k = 1; k < groups; ++k) {
+    const float4 x{__shfl(v.x, lane + k * per), __shfl(v.y, lane + k * per), __shfl(v.z, lane + k * per), __shfl(v.w, lane + k * per)};
+    if (group == 0) v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+  }
+  if (group == 0) {
+    const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = d0 + e;
+      if (d >= a.cache.head_dim) break;
+      if (a.fm != nullptr) a.fm[fm16((int)row, h * a.cache.head_dim + d, a.heads * a.cache.head_dim >> 5)] = ElemOf<Elem::bf16>::put(y[e]);
+      else o[d] = ElemOf<E>::put(y[e]);
+    }
   }
   if (lane == 0 && a.lse != nullptr) a.lse[row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
 }
@@ -490,17 +529,23 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
 template <int M, Elem E>
 void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
   Kv4Attention a = a0;
+  const Kv4Shape shape = kv4_attention_shape(a);
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
   const int64_t pairs = (int64_t)a.batch * a.cache.heads;
-  a.tiles = (int32_t)(rows <= 16 ? 1 : rows <= 64 ? (rows + 31) / 32 : (rows + 127) / 128);
+  a.tiles = (int32_t)((rows + 16 * shape.rt - 1) / (16 * shape.rt));
   const int64_t four = E == Elem::f32 ? 16 : 8;   // bytes of four elements
   const int64_t size = four / 4;
   auto even = [&](const void* p, int64_t row, int64_t head) { return (uintptr_t)p % four == 0 && row * size % four == 0 && head * size % four == 0; };
   a.vec = a.cache.head_dim % 4 == 0 && even(a.q, a.q_row, a.q_head) && (a.fm != nullptr || even(a.out, a.out_row, a.out_head));
-  const dim3 grid((unsigned)(pairs * a.tiles), (unsigned)a.nsplit);
-  if (rows <= 16) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, false>), grid, dim3(256), 0, s, a);
-  else if (rows <= 64) MSH_LAUNCH((kv4_attention_kernel<M, E, 2, false>), grid, dim3(256), 0, s, a);
-  else MSH_LAUNCH((kv4_attention_kernel<M, E, 2, true>), grid, dim3(256), 0, s, a);
+  a.sign = a.scale_log2 < 0.f ? -1.f : 1.f;
+  a.scale_log2 = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);   // (0 * -inf of a masked score would be NaN; any score times this is 0 to exp2)
+  const int64_t per_group = 4 / shape.kw;
+  const dim3 grid((unsigned)((pairs * a.tiles + per_group - 1) / per_group), (unsigned)a.nsplit);
+  if (shape.rt == 1 && shape.kw == 4) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 4>), grid, dim3(256), 0, s, a);
+  else if (shape.rt == 1 && shape.kw == 2) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 2>), grid, dim3(256), 0, s, a);
+  else if (shape.rt == 1) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 1>), grid, dim3(256), 0, s, a);
+  else if (shape.kw == 4) MSH_LAUNCH((kv4_attention_kernel<M, E, 2, 4>), grid, dim3(256), 0, s, a);
+  else MSH_LAUNCH((kv4_attention_kernel<M, E, 2, 1>), grid, dim3(256), 0, s, a);
   if (a.nsplit > 1) MSH_LAUNCH((kv4_join_kernel<E>), dim3((unsigned)((a.rows * a.heads + 3) / 4)), dim3(256), 0, s, a, 32 * M);
 }
 

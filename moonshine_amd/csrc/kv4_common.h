@@ -22,6 +22,16 @@ __device__ inline int kv4_value_scale_at(int t, int g, int m) {
 }
 
 __device__ __forceinline__ float kv4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+// the power of byte B of a word in one instruction: left to itself the compiler shifts and masks
+template <int B>
+__device__ __forceinline__ float kv4_scale_of(uint32_t word) {
+  uint32_t r;
+  if constexpr (B == 0) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (B == 1) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (B == 2) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(word));
+  else asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(word));
+  return __uint_as_float(r);
+}
 
 template <int BYTE>
 __device__ __forceinline__ uint32_t kv4_pair_bf16(uint32_t codes, float scale) {   // exact: one significant bit, a power of two

@@ -58,12 +58,18 @@ struct Kv4Attention {
   Kv4Cache cache;
   int64_t rows;
   int32_t heads, batch, width, max_q, causal, window, nsplit;
-  int32_t tiles, vec;         // set by the launcher
+  int32_t tiles, vec;         // set by the launcher, as is the scale's sign (the kernel's scale is its magnitude)
+  float sign;
   float scale_log2;           // softmax scale * log2(e)
   uint16_t* fm;               // not null: the engine's decode path takes the output as bf16, fragment-major [rows16][heads * head_dim]
                               // (kernels.h fm16), instead of `out`
 };
 constexpr int kPartPad = 4;       // a range's row: 32 m floats, maximum, sum, two unused
+// tile of a wave (16 * rt rows) and waves that share it; see kv4_attention.h
+struct Kv4Shape {
+  int rt, kw;
+};
+Kv4Shape kv4_attention_shape(const Kv4Attention& a);
 // number of key ranges a launch is split into, and the floats of workspace that takes
 int kv4_attention_splits(const Kv4Attention& a, Elem type);
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit);
