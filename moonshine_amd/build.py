@@ -6,7 +6,7 @@
 hipcc cross-compiles gfx950 without a GPU.  Objects go to moonshine_amd/_build/, the library to
 moonshine_amd/lib/libmoonshine.so (git-ignored, but shipped to the GPU box with the tree); beside it
 libmoonshine_dev.so = the same objects + csrc/dev_hooks.cpp (msh_test_*: kernel-alone tests and microbenchmarks),
-which the product library does not export.
+which the product library does not export -- and msh_torch_ops.so, the module behind moonshine_amd.ops.
 """
 from __future__ import annotations
 
@@ -22,7 +22,9 @@ OBJ = os.path.join(HERE, "_build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libmoonshine.so")
 LIB_DEV = os.path.join(LIBDIR, "libmoonshine_dev.so")   # the same objects + the development hooks (include/moonshine_hip_dev.h)
+LIB_OPS = os.path.join(LIBDIR, "msh_torch_ops.so")      # moonshine_amd.ops: the serving operators on torch tensors (a CPython module)
 DEV_ONLY = {"dev_hooks.cpp"}                            # sources that never go into the product library
+TORCH_ONLY = {"torch_ops.cpp"}                          # ... and those that need torch's headers: host code, built beside it
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = "gfx950"
@@ -51,7 +53,7 @@ def hipcc() -> str:
 def sources() -> list[str]:
     out = []
     for f in sorted(os.listdir(CSRC)):
-        if f.endswith(".hip") or f.endswith(".cpp"):
+        if (f.endswith(".hip") or f.endswith(".cpp")) and f not in TORCH_ONLY:
             out.append(os.path.join(CSRC, f))
     return out
 
@@ -128,6 +130,27 @@ def check_no_packed_fp32(objs: list[str]) -> dict[str, int]:
     return seen
 
 
+def build_ops(force: bool = False) -> str:
+    """msh_torch_ops.so: the module behind moonshine_amd.ops.  Host code only; finds libmoonshine.so beside itself."""
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "moonshine_hip.h")))
+    if not force and os.path.exists(LIB_OPS) and os.path.getmtime(LIB_OPS) > newest:
+        return LIB_OPS
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{root}/include",
+           f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", src, "-o", LIB_OPS,
+           f"-L{LIBDIR}", "-l:libmoonshine.so", f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")
+    return LIB_OPS
+
+
 def build(force: bool = False, verbose: bool = False, check: bool = True) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -153,6 +176,7 @@ def build(force: bool = False, verbose: bool = False, check: bool = True) -> str
             r = subprocess.run(cmd, capture_output=True, text=True)
             if r.returncode != 0:
                 raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_ops(force)
     return LIB
 
 

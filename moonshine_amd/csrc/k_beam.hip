@@ -32,7 +32,7 @@ struct Entry {
   float val;
   int idx;
 };
-__host__ __device__ inline size_t part_bytes(int beams) { return sizeof(Part) + sizeof(Entry) * beams; }
+__host__ __device__ inline size_t part_bytes(int beams) { return sizeof(Part) + sizeof(Entry) * ((beams + 1) & ~1); }   // (16-byte multiples)
 
 constexpr int kLane = 32;                                      // elements of a lane per chunk
 constexpr int kListMax = 2 * kBeamMax + kBeamMax * (kLane + 1);   // room for one chunk's most beside 2 K
@@ -87,8 +87,9 @@ __device__ __forceinline__ int rank_list(const Entry* list, Entry* best, int n, 
   return n < K ? n : K;
 }
 
+// (waves per SIMD: at five the 32-bit form spills)
 template <Elem E>
-__global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int parts, uint8_t* work) {
+__global__ __launch_bounds__(256, (E == Elem::f32 ? 4 : 5)) void beam_partial_kernel(BeamSelect a, int parts, uint8_t* work) {
   typedef typename ElemOf<E>::T T;
   constexpr int VEC = 16 / sizeof(T), LOADS = kLane / VEC;
   __shared__ Entry list_s[4][kListMax];
@@ -138,13 +139,20 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
       }
     }
     if (base + 64 * LOADS < v1) fetch(base + 64 * LOADS);
-    const int first = base * VEC + lane * VEC - off;   // index of this lane's element 0; element e: + (e / VEC) * 64 * VEC + e % VEC
-    if (base == 0 || base + 64 * LOADS >= v1) {        // the row's ends and the part's
+    // index of this lane's element 0; element e: + (e / VEC) * 64 * VEC + e % VEC.  (Copies that the compiler takes for different:
+    // otherwise it computes 32 indices once and keeps them in as many registers.)
+    const int first = base * VEC + lane * VEC - off;
+    int first_push = first, first_tie = first;
+    asm("" : "+v"(first_push));
+    asm("" : "+v"(first_tie));
+    if (base == 0 || base + 64 * LOADS >= v1) {        // the row's ends and the part's: places [lo, lo + span) of the chunk count
+      asm volatile("" ::: );
+      const int lo = base == 0 ? off : 0, end = min(v1 * VEC, a.vocab + off) - base * VEC;
+      const uint32_t span = (uint32_t)(end - lo);
+      uint32_t at = (uint32_t)(lane * VEC - lo);
 #pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        const int idx = first + (e / VEC) * 64 * VEC + e % VEC;
-        if (base + (e / VEC) * 64 + lane >= v1 || idx < 0 || idx >= a.vocab) x[e] = -INFINITY;
-      }
+      for (int e = 0; e < kLane; ++e)
+        if (at + (uint32_t)((e / VEC) * 64 * VEC + e % VEC) >= span) x[e] = -INFINITY;
     }
     float hi, group[4], now, part_sum;
     while (true) {
@@ -191,7 +199,7 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
         const bool in = x[e] > bound;
         const uint64_t m = __builtin_amdgcn_ballot_w64(in);
         if (m != 0) {
-          if (in) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = Entry{x[e], first + (e / VEC) * 64 * VEC + e % VEC};
+          if (in) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = Entry{x[e], first_push + (e / VEC) * 64 * VEC + e % VEC};
           n += __popcll(m);
         }
       }
@@ -203,7 +211,7 @@ __global__ __launch_bounds__(256) void beam_partial_kernel(BeamSelect a, int par
         int next = INT_MAX;   // this lane's lowest index behind `after`
 #pragma unroll
         for (int e = kLane - 1; e >= 0; --e) {
-          const int idx = first + (e / VEC) * 64 * VEC + e % VEC;
+          const int idx = first_tie + (e / VEC) * 64 * VEC + e % VEC;
           if (x[e] == bound && idx > after) next = idx;
         }
         int lowest = next;
@@ -234,6 +242,7 @@ struct Pick {
 };
 __device__ __forceinline__ bool before(const Pick& a, const Pick& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
 
+template <int KMAX>
 __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts, const uint8_t* work) {
   __shared__ double offset_s[kBeamMax];
   __shared__ float bound_s[4];
@@ -243,34 +252,47 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
   const int row0 = (int)blockIdx.x * K, stride = (int)part_bytes(K);
   work += (int64_t)row0 * parts * stride;
   if (threadIdx.x == 0) n_s = 0;
-  // score_k - log sum exp of row k, a wave each; -inf: a beam with no candidates of its own (finished, not in use)
-  for (int k = wave; k < K; k += 4) {
-    const float score = a.scores[row0 + k];
+  // everything this workgroup reads, at once: a thread's list (beam, part), best first ...
+  const int k = min((int)threadIdx.x / parts, K - 1), p = (int)threadIdx.x - k * parts;
+  const bool mine = p < parts;
+  const uint4* src = reinterpret_cast<const uint4*>(work + (k * parts + (mine ? p : 0)) * stride + sizeof(Part));
+  Entry list[KMAX];
+#pragma unroll
+  for (int e = 0; e < KMAX; e += 2) {
+    const uint4 u = src[min(e / 2, (K - 1) / 2)];
+    list[e] = Entry{__uint_as_float(u.x), (int)u.y}, list[e + 1] = Entry{__uint_as_float(u.z), (int)u.w};
+  }
+  const float my_score = a.scores[row0 + k];
+  const bool my_end = a.finished[row0 + k] != 0;
+  // ... and a wave's rows: score_k - log sum exp of row k; -inf: a beam with no candidates of its own (finished, not in use)
+  Part q[KMAX / 4];
+#pragma unroll
+  for (int i = 0; i < KMAX / 4; ++i) q[i] = *reinterpret_cast<const Part*>(work + (min(wave + 4 * i, K - 1) * parts + min(lane, parts - 1)) * stride);
+#pragma unroll
+  for (int i = 0; i < KMAX / 4; ++i) {
+    const int row = wave + 4 * i;
+    if (row >= K) break;
+    const float score = a.scores[row0 + row];
     double o = -INFINITY;
-    if (a.finished[row0 + k] == 0 && score > -INFINITY) {
-      Part q{0.0, -INFINITY, 0};
-      if (lane < parts) q = *reinterpret_cast<const Part*>(work + (k * parts + lane) * stride);
-      const float top = wave_max(q.top);
+    if (a.finished[row0 + row] == 0 && score > -INFINITY) {
+      const float part_top = lane < parts ? q[i].top : -INFINITY;
+      const float top = wave_max(part_top);
       // (the differences of the parts' maxima in 64 bits: far below 32 bits' rounding of the exponent)
-      const double sum = wave_sum(q.top == -INFINITY ? 0.0 : q.sum * exp((double)q.top - (double)top));
+      const double sum = wave_sum(part_top == -INFINITY ? 0.0 : q[i].sum * exp((double)part_top - (double)top));
       if (top > -INFINITY) o = (double)score - (log(sum) + (double)top);
     }
-    if (lane == 0) offset_s[k] = o;
+    if (lane == 0) offset_s[row] = o;
   }
   __syncthreads();
-  // a thread holds one list (beam, part), best first; a finished beam's first list is the beam itself
-  const int k = (int)threadIdx.x / parts, p = (int)threadIdx.x - k * parts;
-  double offset = -INFINITY;
-  const Entry* entries = nullptr;
-  int flat0 = k * a.vocab, self = -1;
-  double head = -INFINITY;
-  if (k < K) {
-    offset = offset_s[k];
-    if (a.finished[row0 + k] != 0) {
-      if (p == 0) self = flat0 + (a.eos > 0 ? a.eos : 0), head = (double)a.scores[row0 + k];
-    } else if (offset > -INFINITY) {
-      entries = reinterpret_cast<const Entry*>(work + (k * parts + p) * stride + sizeof(Part));
-      head = offset + (double)entries[0].val;
+  double offset = -INFINITY, head = -INFINITY;
+  const int flat0 = k * a.vocab;
+  int self = -1;   // a finished beam's first list is the beam itself
+  if (mine) {
+    if (my_end) {
+      if (p == 0) self = flat0 + (a.eos > 0 ? a.eos : 0), head = (double)my_score;
+    } else {
+      offset = offset_s[k];
+      if (offset > -INFINITY) head = offset + (double)list[0].val;
     }
   }
   const float kth = wave_kth((float)head, K, lane);
@@ -280,13 +302,11 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
   auto add = [&](double score, int flat) { list_s[atomicAdd(&n_s, 1)] = Pick{score, flat, 0}; };   // (any order: it is ranked below)
   if (self >= 0) {
     if (head > -INFINITY && (float)head >= bound) add(head, self);
-  } else if (entries != nullptr) {
-#pragma unroll 1
-    for (int e = 0; e < K; ++e) {
-      const Entry en = entries[e];
-      const double v = offset + (double)en.val;
-      if (!(en.val > -INFINITY) || (float)v < bound) break;
-      add(v, flat0 + en.idx);
+  } else if (offset > -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < KMAX; ++e) {
+      const double v = offset + (double)list[e].val;
+      if (e < K && list[e].val > -INFINITY && (float)v >= bound) add(v, flat0 + list[e].idx);
     }
   }
   __syncthreads();
@@ -299,15 +319,15 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
   };
 #pragma unroll 1
   for (int i = threadIdx.x; i < n; i += 256) {
-    const Pick mine = list_s[i];
+    const Pick one = list_s[i];
     int rank = 0;
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) rank += before(list_s[j], mine) ? 1 : 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += before(list_s[j], one) ? 1 : 0;
     if (rank < K) {
-      const int parent = mine.flat / a.vocab;
+      const int parent = one.flat / a.vocab;
       const bool over = a.finished[row0 + parent] != 0;
-      const int token = over ? a.eos : mine.flat - parent * a.vocab;
-      put(rank, mine.score, parent, token, over || token == a.eos);
+      const int token = over ? a.eos : one.flat - parent * a.vocab;
+      put(rank, one.score, parent, token, over || token == a.eos);
     }
   }
   if ((int)threadIdx.x >= n && (int)threadIdx.x < K) put(threadIdx.x, -INFINITY, threadIdx.x, a.eos, true);   // too few candidates
@@ -316,8 +336,7 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
 // parts of a row: enough waves to fill the chip, at least a chunk each, and lists that pass 2 holds at one a thread
 int beam_parts(int batch, int beams, int vocab) {
   const int64_t rows = (int64_t)batch * beams;
-  static const char* env = getenv("BPN");
-  int64_t n = ((env ? atoi(env) : 8192) + rows - 1) / rows;
+  int64_t n = (12288 + rows - 1) / rows;
   const int64_t chunks = (vocab + 64 * kLane - 1) / (64 * kLane);
   n = n < chunks ? n : chunks;
   const int64_t most = kPicks / (beams * beams);
@@ -459,7 +478,9 @@ void beam_select(const BeamSelect& a, Elem type, hipStream_t s) {
   if (type == Elem::f32) MSH_LAUNCH((beam_partial_kernel<Elem::f32>), grid, dim3(256), 0, s, a, parts, work);
   else if (type == Elem::bf16) MSH_LAUNCH((beam_partial_kernel<Elem::bf16>), grid, dim3(256), 0, s, a, parts, work);
   else MSH_LAUNCH((beam_partial_kernel<Elem::f16>), grid, dim3(256), 0, s, a, parts, work);
-  MSH_LAUNCH(beam_pick_kernel, dim3(a.batch), dim3(256), 0, s, a, parts, work);
+  if (a.beams <= 4) MSH_LAUNCH(beam_pick_kernel<4>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
+  else if (a.beams <= 8) MSH_LAUNCH(beam_pick_kernel<8>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
+  else MSH_LAUNCH(beam_pick_kernel<16>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
 }
 
 void beam_reorder(const BeamState* states, int n_states, int batch, int beams, const int32_t* parents, const int32_t* lengths,

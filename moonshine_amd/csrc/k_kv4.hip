@@ -324,11 +324,9 @@ void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 // Rows of one key / value head: up to 16 one tile, above that tiles of 32.  Waves share a tile while there are too few tiles to fill the chip
 // (1024 SIMDs) without.
 Kv4Shape kv4_attention_shape(const Kv4Attention& a) {
-  static const char* env = getenv("KV4_SHAPE");
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
   const int rt = rows <= 16 ? 1 : 2;
   const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + 16 * rt - 1) / (16 * rt));
-  if (env && rt == 1) return Kv4Shape{1, atoi(env)};
   if (rt == 2) return Kv4Shape{2, rows > 64 ? 1 : 4};
   return Kv4Shape{1, units >= 4096 ? 1 : units >= 2048 ? 2 : 4};
 }
@@ -342,9 +340,7 @@ int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   const int64_t groups = (int64_t)a.batch * a.cache.heads * ((rows + 16 * shape.rt - 1) / (16 * shape.rt));
   const int64_t room = (int64_t)a.width << a.cache.page_shift;
   const int64_t most = room / 512;   // four blocks per wave at least: a block takes a wave about 1 us, the second launch 3
-  static const char* env = getenv("KV4_WG");
-  const int64_t want = env ? atoi(env) : 2048;
-  int64_t n = (want + groups - 1) / groups;
+  int64_t n = (2048 + groups - 1) / groups;
   n = n < most ? n : most;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }

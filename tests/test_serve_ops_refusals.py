@@ -1,5 +1,6 @@
 """What the serving operators refuse, on the CPU: every refusal comes before anything touches a device, so none of these needs one."""
 import ctypes as C
+import struct
 
 import numpy as np
 import pytest
@@ -9,6 +10,10 @@ import serve_ref
 from moonshine_amd import ops
 from moonshine_amd.hip_api import MshError, load_library
 
+CACHE = struct.Struct("Pqiiixxxx")                        # msh_kv4_cache
+ATTENTION = struct.Struct("PPPqqqqPPPPqiiixxxxqiiiiiiif")   # msh_kv4_attention_args
+STATE = struct.Struct("Pqqqqqqq")                         # msh_beam_state
+STRIDES = struct.Struct("qqq")
 FAKE = 1 << 20   # a 16-byte aligned address that nothing reads
 
 
@@ -17,7 +22,7 @@ def _attention(**change):
              kv_heads=1, page=32, width=64, rows=2, dtype=0, heads=1, batch=2, table_width=2, max_q=1, causal=1, window=0, scale=1.0)
     assert set(change) <= set(a)
     a.update(change)
-    return ops._ATTENTION.pack(*a.values())
+    return ATTENTION.pack(*a.values())
 
 
 @pytest.mark.parametrize("change, says", [
@@ -49,7 +54,7 @@ def test_nothing_to_do_is_no_error():
     """Empty calls return before they touch a device."""
     lib = load_library()
     assert lib.msh_kv4_attention(0, None, _attention(rows=0, batch=0, q=0), None, 0) == 0
-    cache = ops._CACHE.pack(FAKE, 4, 1, 32, 64)
+    cache = CACHE.pack(FAKE, 4, 1, 32, 64)
     assert lib.msh_kv4_write(0, None, cache, None, None, None, None, 0, 0, None) == 0
     assert lib.msh_kv4_read(0, None, cache, None, 0, None, None, 0) == 0
     assert lib.msh_beam_select_workspace(0, 4, 100) == 0
@@ -68,10 +73,10 @@ def test_plan_write_select_reorder_refuse():
                      (dict(n_free=-1), "n_free"), (dict(table=None), "null"), (dict(slots=None), "null"), (dict(width=1 << 26), "table_width")):
         rc, msg = plan(**kw)
         assert rc == -3 and word in msg
-    strides = ops._STRIDES.pack(64, 64, 1)
+    strides = STRIDES.pack(64, 64, 1)
 
     def write(pages=4, heads=1, page=32, width=64, dtype=0, rows=2, k=FAKE):
-        return says(lib.msh_kv4_write(0, None, ops._CACHE.pack(FAKE, pages, heads, page, width), k, strides, FAKE, strides, dtype, rows, FAKE))
+        return says(lib.msh_kv4_write(0, None, CACHE.pack(FAKE, pages, heads, page, width), k, strides, FAKE, strides, dtype, rows, FAKE))
 
     for kw, word in ((dict(pages=0), "pages"), (dict(heads=0), "heads"), (dict(page=40), "page_size"), (dict(width=300), "head_dim"),
                      (dict(dtype=-1), "dtype"), (dict(rows=-1), "rows"), (dict(rows=1 << 40), "rows"), (dict(k=None), "null")):
@@ -88,7 +93,7 @@ def test_plan_write_select_reorder_refuse():
         assert rc == -3 and word in msg
 
     def reorder(n=1, batch=1, beams=2, lstride=0, parents=FAKE, data=FAKE, outer=1, outer_stride=0, beam_stride=64, inner=1, inner_stride=0, row_bytes=8, n_rows=8):
-        state = ops._STATE.pack(data, outer, outer_stride, beam_stride, inner, inner_stride, row_bytes, n_rows)
+        state = STATE.pack(data, outer, outer_stride, beam_stride, inner, inner_stride, row_bytes, n_rows)
         return says(lib.msh_beam_reorder(0, None, state * max(n, 1), n, batch, beams, parents, None, lstride))
 
     for kw, word in ((dict(n=5), "states"), (dict(n=-1), "states"), (dict(beams=17), "beams"), (dict(beams=0), "beams"), (dict(lstride=2), "length_stride"),
@@ -162,6 +167,6 @@ def test_ctypes_structs_match_the_header():
         _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("s", C.c_int64 * 4), ("t", C.c_void_p * 3), ("cache", Cache),
                     ("rows", C.c_int64), ("i", C.c_int32 * 7), ("scale", C.c_float)]
 
-    assert C.sizeof(Cache) == ops._CACHE.size and C.sizeof(Attention) == ops._ATTENTION.size and ops._STATE.size == 64
+    assert C.sizeof(Cache) == CACHE.size and C.sizeof(Attention) == ATTENTION.size and STATE.size == 64
     raw = Attention.from_buffer_copy(_attention(scale=0.5, window=7))
     assert raw.scale == 0.5 and raw.i[6] == 7 and raw.cache.head_dim == 64 and raw.rows == 2
