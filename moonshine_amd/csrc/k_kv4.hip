@@ -321,28 +321,44 @@ void kv4_attention_f32(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_bf16(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 
-// Rows of one key / value head: up to 16 one tile, above that tiles of 32.  Waves share a tile while there are too few tiles to fill the chip
-// (1024 SIMDs) without.
-Kv4Shape kv4_attention_shape(const Kv4Attention& a) {
-  const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
-  const int rt = rows <= 16 ? 1 : 2;
-  const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + 16 * rt - 1) / (16 * rt));
-  if (rt == 2) return Kv4Shape{2, rows > 64 ? 1 : 4};
-  return Kv4Shape{1, units >= 4096 ? 1 : units >= 2048 ? 2 : 4};
+// Which form, by the rows of one key / value head and the work there is (times of 32 query over 8 key / value heads of 128, bf16, in us):
+// * more than 64 rows: the form for chunks once its units of 128 rows fill the chip's 512 places (2048 tokens: 2 x 1024 queries 112 against 120 by
+//   tiles of 32, 64 sequences of 512 with 128 queries each 133 against 202; half as many units: 1 x 1024 queries 80 against 70).
+// * 17 rows and more: tiles of 32 (32 sequences of 2048, 64 rows: 38 against 49 by tiles of 16), but for 32-bit rows of more than 96, which spill
+//   (64 rows: 70 by tiles of 16 against 76, 256 rows 246 against 294).
+// * tiles of 16: all four waves of a workgroup share a tile as long as there are too few to fill the chip without, then two, then none -- a wave's beginning
+//   and end cost as much as three blocks, so sooner for short tables (units, KW 4 / 2 / 1; 100 tokens: 1024 units 9.9 / 8.0 / 8.2, 3072 units
+//   23.6 / 17.1 / 15.3; 2048 tokens: 1280 units 55 / 62 / 85, 4096 units 191 / 181 / 184).
+Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
+  const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads), pairs = (int64_t)a.batch * a.cache.heads;
+  if (rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
+  if (rows > 16 && !(type == Elem::f32 && a.cache.head_dim > 96)) return Kv4Shape{2, 4, false};
+  const int64_t units = pairs * ((rows + 15) / 16), room = (int64_t)a.width << a.cache.page_shift;
+  const bool brief = room <= 1024;
+  return Kv4Shape{1, units >= (brief ? 2560 : 4096) ? 1 : units >= (brief ? 1024 : 2048) ? 2 : 4, false};
 }
 
-// The lengths live on the device; the host knows the table's room only.  A range is a share of each sequence's own length, so a short
-// sequence in a wide table costs empty ranges and nothing else.
+// Key ranges, joined by a second launch (4 to 40 us, by the rows).  The lengths live on the device; the host knows the table's room only.  A
+// range is a share of each sequence's own length, so a short sequence in a wide table costs empty ranges and nothing else.
+// Few units: as many ranges as fill the chip, none of them shorter than pays for its share of the join (single tokens, units x tokens, ranges 1 / 2 /
+// 4 / 8 / 16 / 32: 8 x 1024: 11 / 10 / 9.1 / 8.5 / 9.0 / 10; 64 x 4096: 29 / 20 / 15 / 14 / 17 / 24; 128 x 16384: 107 / 61 / 51 / 49 / 52 / 62, but with
+// lengths between 1500 and 16383 161 at 2, 116 at 8 and 106 at 16; 512 x 4096: 47 / 49 / 52 / 59; 32-row tiles: 32 x 8192: 73 / 44 / 29 / 22 / 26 / 34;
+// 256 x 2048: 27 / 32).  Below 1024 tokens one (8 units x 600: 8.4 / 9.7).
+// Chunks: two ranges where units are few enough for long and short sequences to leave places empty at the end (4 sequences of 2500 to 8191 tokens,
+// 485 to 1000 queries: 529 against 617; all of 8192: 771 against 752; at 2048 tokens the join would cost a quarter: 260 against 207).
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
-  const Kv4Shape shape = kv4_attention_shape(a);
-  if (shape.kw != 4) return 1;
+  const Kv4Shape shape = kv4_attention_shape(a, type);
+  if (shape.kw != 4 || a.rows * a.heads >= (1 << 26)) return 1;   // (a grid has 2^32 threads)
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
-  const int64_t groups = (int64_t)a.batch * a.cache.heads * ((rows + 16 * shape.rt - 1) / (16 * shape.rt));
+  const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + shape.rows() - 1) / shape.rows());
   const int64_t room = (int64_t)a.width << a.cache.page_shift;
-  const int64_t most = room / 512;   // four blocks per wave at least: a block takes a wave about 1 us, the second launch 3
-  int64_t n = (2048 + groups - 1) / groups;
-  n = n < most ? n : most;
-  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  if (shape.chunk) return units < 1536 && room >= 8192 ? 2 : 1;
+  if (room < 1024) return 1;
+  const int64_t wanted = shape.rt == 2 ? 512 : room < 16384 ? 1024 : 2048;
+  const int64_t least = units <= 32 ? 256 : (units <= 128 ? 512 : 1024) * shape.rt;
+  int64_t n = wanted / units;
+  n = n < room / least ? n : room / least;
+  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit) {
   return nsplit > 1 ? (size_t)a.rows * a.heads * nsplit * (32 * kv4_groups(a.cache.head_dim) + kPartPad) : 0;

@@ -87,7 +87,7 @@ msh::Kv4Attention attention_of(const msh_kv4_attention_args* x, msh::Elem* type)
   const int64_t per = x->heads / a.cache.heads;
   need((int64_t)x->max_q * per <= kMost, "max_q * heads per cache head: at most 2^30");
   const int64_t tiles = ((int64_t)x->max_q * per + 15) / 16;
-  need((int64_t)x->batch * a.cache.heads * tiles < ((int64_t)1 << 31) && x->rows * x->heads < ((int64_t)1 << 32), "the call is too large for one launch");
+  need((double)x->batch * a.cache.heads * tiles < (1 << 24) && x->rows * x->heads < ((int64_t)1 << 32), "the call is too large for one launch");
   a.q = x->q, a.out = x->out, a.lse = x->lse;
   a.q_row = x->q_row_stride, a.q_head = x->q_head_stride, a.out_row = x->out_row_stride, a.out_head = x->out_head_stride;
   a.table = x->block_table, a.kv_lens = x->kv_lens, a.q_start = x->q_start;

@@ -65,11 +65,13 @@ struct Kv4Attention {
                               // (kernels.h fm16), instead of `out`
 };
 constexpr int kPartPad = 4;       // a range's row: 32 m floats, maximum, sum, two unused
-// tile of a wave (16 * rt rows) and waves that share it; see kv4_attention.h
+// tile of a wave (16 * rt rows) and waves that share it, or the form for chunks of prompts; see kv4_attention.h
 struct Kv4Shape {
   int rt, kw;
+  bool chunk;
+  int rows() const { return 16 * rt * (chunk ? 4 : 1); }   // of a unit of work
 };
-Kv4Shape kv4_attention_shape(const Kv4Attention& a);
+Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type);
 // number of key ranges a launch is split into, and the floats of workspace that takes
 int kv4_attention_splits(const Kv4Attention& a, Elem type);
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit);

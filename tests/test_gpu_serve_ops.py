@@ -238,6 +238,57 @@ def test_attention_long_is_split_and_joined(dtype, batch, heads, kv_heads, width
     check_attention(dtype, heads, kv_heads, width, 64, lengths, [3] * batch, window=n // 2, seed=10)
 
 
+@pytest.mark.parametrize("width", [32, 96, 128, 256])
+def test_attention_many_ranges(width):
+    """More key ranges than an eighth or a half of a wave, also odd numbers of them: each must find its weight when they are joined."""
+    for others in (3, 58):
+        check_attention("bf16", 1, 1, width, 64, [18000] + ([300, 0, 7] * 20)[:others], [1] * (others + 1), uniform=True, seed=11)
+    check_attention("bf16", 2, 2, width, 64, [7400, 33], [1, 1], uniform=True, seed=12)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_long_chunks(dtype, window):
+    """Chunks of prompts behind long beginnings: key ranges are split here too, some of them with nothing that a row sees."""
+    check_attention(dtype, 4, 2, 128, 64, [3000, 700, 40, 0], [300, 33, 40, 2], window=window, seed=12)
+    check_attention(dtype, 2, 2, 52, 32, [2111], [129], causal=window > 0, window=window, seed=13)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("heads, kv_heads, width, page", [(8, 8, 52, 32), (8, 8, 32, 64), (16, 8, 128, 64), (24, 8, 96, 32), (8, 8, 160, 32), (8, 8, 224, 32), (8, 8, 256, 128)])
+@pytest.mark.parametrize("causal, window", [(True, 0), (False, 0), (True, 37)])
+def test_attention_batches_of_chunks(dtype, heads, kv_heads, width, page, causal, window):
+    """A batch with room for enough prompts that a block is expanded once for four waves: whole and broken tiles, more rows than tokens,
+    sequences without rows or tokens."""
+    counts, lengths = [70, 0, 128, 1, 0, 129, 65] + [0] * 57 + [30, 90], [300, 64, 150, 203, 1, 0, 33] + [0] * 57 + [97, 64]
+    check_attention(dtype, heads, kv_heads, width, page, lengths, counts, causal, window, seed=14)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("window", [0, 5000])
+def test_attention_batches_of_long_chunks(dtype, window):
+    """The same with key ranges of two workgroups, one sequence far longer than the others."""
+    check_attention(dtype, 8, 8, 64, 64, [8200, 100, 0, 33] + [40] * 60, [70, 70, 3, 65] + [7] + [0] * 59, window=window, seed=15)
+
+
+def test_attention_chunks_with_pages_that_are_not_there():
+    """A page outside the cache counts as absent in every form: its tokens get no weight."""
+    batch, rows, n = 64, 70, 160
+    k, v = values(gen(3), (batch * 5, 8, 32, 64)), values(gen(4), (batch * 5, 8, 32, 64))
+    cache = ops.kv4_cache(batch * 5, 8, 32, 64)
+    slots = torch.arange(batch * 160, device="cuda")
+    ops.kv4_write(cache, dev(np.ascontiguousarray(k.transpose(0, 2, 1, 3)).reshape(-1, 8, 64)), dev(np.ascontiguousarray(v.transpose(0, 2, 1, 3)).reshape(-1, 8, 64)), slots)
+    table = torch.arange(batch * 5, dtype=torch.int32, device="cuda").view(batch, 5).clone()
+    q = dev(values(gen(5), (batch * rows, 8, 64)), torch.bfloat16)
+    lens = i32([n] * batch)
+    bad = table.clone()
+    bad[:, 1], bad[:, 3] = -1, batch * 5
+    out = ops.kv4_attention(q, cache, bad, lens, max_q=rows, causal=False)
+    short = table[:, [0, 2, 4]].contiguous()
+    want = ops.kv4_attention(q, cache, short, i32([96] * batch), max_q=rows, causal=False)
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_attention_sharp_and_flat_rows(dtype):
     """Scores of hundreds (one token takes all; the running maximum moves often) and of nothing."""
