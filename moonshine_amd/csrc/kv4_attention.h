@@ -106,18 +106,22 @@ struct BlockBytes {
     }
     expand_values(v + 2 * g, s, even, odd);
   }
+  // (A uniform address and 32-bit offsets of the lane: one register an offset, no 64-bit additions.  The empty asm keeps the compiler from widening them
+  // outside of the loop.)
   __device__ __forceinline__ void load(const uint8_t* b, int lane) {
-    const int quarter = lane >> 4, idx = lane & 15;
+    uint32_t quarter = (uint32_t)lane >> 4, idx = lane & 15, lane4 = lane * 4;
+    asm("" : "+v"(quarter));
+    asm("" : "+v"(idx));
+    asm("" : "+v"(lane4));
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
-      const uint8_t* p = b + tile * 256 * M;
       if constexpr (M <= 4) {
-        load_dwords<M>(p + lane * 4 * M, k[tile]);
+        load_dwords<M>(b + lane4 * M + tile * 256 * M, k[tile]);
       } else {
-        load_dwords<4>(p + lane * 16, k[tile]);
-        load_dwords<M - 4>(p + 1024 + lane * 4 * (M - 4), k[tile] + 4);
+        load_dwords<4>(b + lane4 * 4 + tile * 256 * M, k[tile]);
+        load_dwords<M - 4>(b + lane4 * (M - 4) + (tile * 256 * M + 1024), k[tile] + 4);
       }
-      const uint8_t* q = b + 512 * M + (tile * 16 + idx) * M;
+      const uint8_t* q = b + idx * M + (512 + tile * 16) * M;
       if constexpr (M % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < M / 4; ++i) ks[tile][i] = reinterpret_cast<const uint32_t*>(q)[i];
@@ -133,17 +137,17 @@ struct BlockBytes {
         for (int i = 0; i < M; ++i) ks[tile][i / 4] |= (uint32_t)q[i] << (8 * (i & 3));
       }
     }
-    const uint8_t* p = b + 544 * M;
 #pragma unroll
-    for (int c = 0; c < M / 2; ++c) load_dwords<4>(p + c * 1024 + lane * 16, v + 4 * c);
-    if constexpr (M % 2 == 1) load_dwords<2>(p + (M / 2) * 1024 + lane * 8, v + 2 * (M - 1));
-    const uint8_t* s = b + 1056 * M + quarter * 8 * M;
-    if constexpr (M % 2 == 0) {
+    for (int c = 0; c < M / 2; ++c) load_dwords<4>(b + lane4 * 4 + (544 * M + c * 1024), v + 4 * c);
+    if constexpr (M % 2 == 1) load_dwords<2>(b + lane4 * 2 + (544 * M + M / 2 * 1024), v + 2 * (M - 1));
 #pragma unroll
-      for (int i = 0; i < M / 2; ++i) load_dwords<4>(s + 16 * i, vs + 4 * i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < M; ++i) load_dwords<2>(s + 8 * i, vs + 2 * i);
+    for (int i = 0; i < M; i += 2) {
+      if constexpr (M % 2 == 0) {
+        load_dwords<4>(b + quarter * 8 * M + (1056 * M + 8 * i), vs + 2 * i);
+      } else {
+        load_dwords<2>(b + quarter * 8 * M + (1056 * M + 8 * i), vs + 2 * i);
+        if (i + 1 < M) load_dwords<2>(b + quarter * 8 * M + (1056 * M + 8 * i + 8), vs + 2 * i + 2);
+      }
     }
   }
 };
@@ -222,13 +226,14 @@ struct Walk {
       for (int rt = 0; rt < RT; ++rt) s[rt][tile] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < M; ++g) {
-      const Frag k[2] = {b.keys(0, g), b.keys(1, g)};
 #pragma unroll
-      for (int w = QT - 1; w >= 0; --w)   // small terms first
+      for (int tile = 0; tile < 2; ++tile) {
+        const Frag k = b.keys(tile, g);
 #pragma unroll
-        for (int tile = 0; tile < 2; ++tile)
+        for (int w = QT - 1; w >= 0; --w)   // small terms first
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][tile] = mma(k[tile], q[rt][g][w], s[rt][tile]);
+          for (int rt = 0; rt < RT; ++rt) s[rt][tile] = mma(k, q[rt][g][w], s[rt][tile]);
+      }
     }
   }
   // what a row does not see of the block from t0 on; window: tokens up to its last one that it sees (0: all)
@@ -412,10 +417,19 @@ __global__ __launch_bounds__(256, (waves_wanted<M, E, RT>())) void kv4_attention
   const int32_t* table = a.table + (int64_t)b * a.width;
   const int64_t block_bytes = kv4_block_bytes(M);
   const int in_shift = page_shift - 5, in_mask = (1 << in_shift) - 1;
+  // 64 entries of the table at a time, one a lane: a load of each would be waited for in every turn
+  const int last_page = (blk1 - 1) >> in_shift;
+  int held = blk0 >> in_shift;
+  int32_t entries = blk0 < blk1 ? table[min(held + lane, last_page)] : -1;
   // (blocks behind the last are the last again, and a page that is not in the cache is page 0, not looked at: the loads of a step are
   // unconditional, or each would be waited for where its condition ends)
-  auto page_of = [&](int blk) -> int32_t { return table[(blk < blk1 ? blk : blk1 - 1) >> in_shift]; };
-  auto good = [&](int32_t page) { return page >= 0 && page < a.cache.pages; };
+  auto page_of = [&](int blk) -> int32_t {
+    const int i = min(blk, blk1 - 1) >> in_shift;
+    if (i - held >= 64) held = i, entries = table[min(held + lane, last_page)];
+    return __builtin_amdgcn_readlane(entries, i - held);
+  };
+  const uint32_t pages = a.cache.pages < INT_MAX ? (uint32_t)a.cache.pages : (uint32_t)INT_MAX;
+  auto good = [&](int32_t page) { return (uint32_t)page < pages; };
   auto at = [&](int blk, int32_t page) {
     return a.cache.data + ((((int64_t)(good(page) ? page : 0) * heads_kv + head) << in_shift) + ((blk < blk1 ? blk : blk1 - 1) & in_mask)) * block_bytes;
   };
@@ -510,8 +524,8 @@ struct QuarterKeys {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int f = min(wave + 4 * i, 2 * M - 1), tile = f / M, g = f - tile * M;
-      k[i] = *reinterpret_cast<const uint32_t*>(b + kv4_key_at(tile * 16 + idx, g, quarter, M));
-      s[i] = b[kv4_key_scale_at(tile * 16 + idx, g, M)];
+      k[i] = *reinterpret_cast<const uint32_t*>(b + (uint32_t)kv4_key_at(tile * 16 + idx, g, quarter, M));
+      s[i] = b[(uint32_t)kv4_key_scale_at(tile * 16 + idx, g, M)];
     }
   }
   __device__ __forceinline__ void expand(Frag* f, int wave, int i) const {
@@ -528,8 +542,8 @@ struct QuarterValues {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int g = min(((wave + 2) & 3) + 4 * i, M - 1);
-      v[i] = *reinterpret_cast<const uint2*>(b + kv4_value_at(quarter * 4, g, idx, M));
-      s[i] = *reinterpret_cast<const uint2*>(b + kv4_value_scale_at(quarter * 4, g, M));
+      v[i] = *reinterpret_cast<const uint2*>(b + (uint32_t)kv4_value_at(quarter * 4, g, idx, M));
+      s[i] = *reinterpret_cast<const uint2*>(b + (uint32_t)kv4_value_scale_at(quarter * 4, g, M));
     }
   }
   __device__ __forceinline__ void expand(Frag* f, int wave, const uint32_t* keep, int i) const {
@@ -602,7 +616,8 @@ __global__ __attribute__((amdgpu_waves_per_eu((M <= 4 ? 2 : 1), (M <= 4 ? 2 : 1)
     if (i - held >= 64) held = i, entries = table[min(held + lane, last_page)];
     return __builtin_amdgcn_readlane(entries, i - held);
   };
-  auto good = [&](int32_t page) { return page >= 0 && page < a.cache.pages; };
+  const uint32_t pages = a.cache.pages < INT_MAX ? (uint32_t)a.cache.pages : (uint32_t)INT_MAX;
+  auto good = [&](int32_t page) { return (uint32_t)page < pages; };
   auto at = [&](int blk, int32_t page) {   // (a page that is not in the cache: page 0, not looked at)
     return a.cache.data + ((((int64_t)(good(page) ? page : 0) * heads_kv + head) << in_shift) + (min(blk, blk1 - 1) & in_mask)) * block_bytes;
   };
