@@ -19,8 +19,10 @@ __device__ __forceinline__ void wave_fence() {   // shared memory written by one
 //   the 64 lanes' maxima bounds the K-th largest element from below, so that all but a handful are dismissed by one comparison;
 //   later elements are held against that bound, and the list of what passed is ranked once.  One read of the logits: bound by HBM bandwidth for batches, by
 //   latency (and the fetch of its own instructions: rare paths are loops, not copies) for one clip.
-// Pass 2, one workgroup per batch entry: joins the rows' sums, takes from the parts' lists what reaches the K-th largest list head,
-//   ranks those few by counting.
+// Pass 2, one workgroup per batch entry, a thread per (row, part): joins the rows' sums, takes from the parts' lists what reaches the K-th
+//   largest list head of a wave, ranks those few by counting.  Bound by the latency of its chain of steps.
+// 256 entries of 8 beams over 32768 bf16 logits (a sixth of the beams finished: 114 MB): 40 us, 2.8 TB/s, and 9.6 us; 1 entry of 4 beams, 32-bit logits:
+// 6.9 and 3.9 us; 1 entry of 7 beams over 193001: 11 and 6 us.
 // The sums are added in 64 bits from 32 exponentials at a time and the scores compared in 64 bits: the order of two candidates of
 // different beams hangs on both rows' sums.
 struct Part {
@@ -36,8 +38,7 @@ __host__ __device__ inline size_t part_bytes(int beams) { return sizeof(Part) + 
 
 constexpr int kLane = 32;                                      // elements of a lane per chunk
 constexpr int kListMax = 2 * kBeamMax + kBeamMax * (kLane + 1);   // room for one chunk's most beside 2 K
-constexpr int kPartsMax = 64;                                  // a wave of pass 2 joins a row's parts
-constexpr int kPicks = 1024;                                   // beams * parts * beams at most
+constexpr int kPartsMax = 64;                                  // a row's parts lie in one wave of pass 2
 
 __device__ __forceinline__ bool before(const Entry& a, const Entry& b) { return a.val > b.val || (a.val == b.val && a.idx < b.idx); }
 
@@ -235,27 +236,26 @@ __global__ __launch_bounds__(256, (E == Elem::f32 ? 4 : 5)) void beam_partial_ke
   if (lane < K) reinterpret_cast<Entry*>(out + sizeof(Part))[lane] = lane < have ? best[lane] : Entry{-INFINITY, INT_MAX};
 }
 
-struct Pick {
-  double score;
-  int flat;   // beam * vocab + id: below 2^28
-  int pad;
-};
-__device__ __forceinline__ bool before(const Pick& a, const Pick& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
+// T threads: 256, or 512 where there are more than 256 lists or 1024 possible candidates.  `shift`: a row's lists lie in 2^shift lanes of one wave.
+constexpr int picks_of(int threads) { return threads == 256 ? 1024 : 4096; }
 
-template <int KMAX>
-__global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts, const uint8_t* work) {
-  __shared__ double offset_s[kBeamMax];
-  __shared__ float bound_s[4];
-  __shared__ Pick list_s[kPicks];
+template <int KMAX, int T>
+__global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelect a, int parts, int shift, const uint8_t* work) {
+  __shared__ float bound_s[T / 64];
+  __shared__ double score_s[picks_of(T)];   // candidates: the score and beam * vocab + id, below 2^28
+  __shared__ int flat_s[picks_of(T)];
+  __shared__ uint8_t end_s[kBeamMax];
   __shared__ int n_s;
   const int K = a.beams, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row0 = (int)blockIdx.x * K, stride = (int)part_bytes(K);
   work += (int64_t)row0 * parts * stride;
   if (threadIdx.x == 0) n_s = 0;
-  // everything this workgroup reads, at once: a thread's list (beam, part), best first ...
-  const int k = min((int)threadIdx.x / parts, K - 1), p = (int)threadIdx.x - k * parts;
-  const bool mine = p < parts;
-  const uint4* src = reinterpret_cast<const uint4*>(work + (k * parts + (mine ? p : 0)) * stride + sizeof(Part));
+  // everything this workgroup reads, at once: a thread's list (beam, part), best first, and the part's sum
+  const int k = min((int)threadIdx.x >> shift, K - 1), p = (int)threadIdx.x & ((1 << shift) - 1);
+  const bool mine = (int)threadIdx.x >> shift < K && p < parts;
+  const uint8_t* from = work + (k * parts + (mine ? p : 0)) * stride;
+  const Part q = *reinterpret_cast<const Part*>(from);
+  const uint4* src = reinterpret_cast<const uint4*>(from + sizeof(Part));
   Entry list[KMAX];
 #pragma unroll
   for (int e = 0; e < KMAX; e += 2) {
@@ -264,42 +264,37 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
   }
   const float my_score = a.scores[row0 + k];
   const bool my_end = a.finished[row0 + k] != 0;
-  // ... and a wave's rows: score_k - log sum exp of row k; -inf: a beam with no candidates of its own (finished, not in use)
-  Part q[KMAX / 4];
-#pragma unroll
-  for (int i = 0; i < KMAX / 4; ++i) q[i] = *reinterpret_cast<const Part*>(work + (min(wave + 4 * i, K - 1) * parts + min(lane, parts - 1)) * stride);
-#pragma unroll
-  for (int i = 0; i < KMAX / 4; ++i) {
-    const int row = wave + 4 * i;
-    if (row >= K) break;
-    const float score = a.scores[row0 + row];
-    double o = -INFINITY;
-    if (a.finished[row0 + row] == 0 && score > -INFINITY) {
-      const float part_top = lane < parts ? q[i].top : -INFINITY;
-      const float top = wave_max(part_top);
-      // (the differences of the parts' maxima in 64 bits: far below 32 bits' rounding of the exponent)
-      const double sum = wave_sum(part_top == -INFINITY ? 0.0 : q[i].sum * exp((double)part_top - (double)top));
-      if (top > -INFINITY) o = (double)score - (log(sum) + (double)top);
-    }
-    if (lane == 0) offset_s[row] = o;
-  }
-  __syncthreads();
+  if (p == 0) end_s[k] = my_end;
+  // score_k - log sum exp of row k; -inf: a beam with no candidates of its own (finished, not in use).  (The differences of the parts' maxima
+  // in 64 bits: far below 32 bits' rounding of the exponent.)
+  const float part_top = mine && !my_end && my_score > -INFINITY ? q.top : -INFINITY;
+  float top = part_top;
+#pragma unroll 1
+  for (int o = 0; o < shift; ++o) top = fmaxf(top, __shfl_xor(top, 1 << o));
+  double sum = part_top == -INFINITY ? 0.0 : q.sum * exp((double)part_top - (double)top);
+#pragma unroll 1
+  for (int o = 0; o < shift; ++o) sum += __shfl_xor(sum, 1 << o);
   double offset = -INFINITY, head = -INFINITY;
   const int flat0 = k * a.vocab;
   int self = -1;   // a finished beam's first list is the beam itself
   if (mine) {
     if (my_end) {
       if (p == 0) self = flat0 + (a.eos > 0 ? a.eos : 0), head = (double)my_score;
-    } else {
-      offset = offset_s[k];
-      if (offset > -INFINITY) head = offset + (double)list[0].val;
+    } else if (top > -INFINITY) {
+      offset = (double)my_score - (log(sum) + (double)top);
+      head = offset + (double)list[0].val;
     }
   }
   const float kth = wave_kth((float)head, K, lane);
   if (lane == 0) bound_s[wave] = kth;
   __syncthreads();
-  const float bound = fmaxf(fmaxf(bound_s[0], bound_s[1]), fmaxf(bound_s[2], bound_s[3]));
-  auto add = [&](double score, int flat) { list_s[atomicAdd(&n_s, 1)] = Pick{score, flat, 0}; };   // (any order: it is ranked below)
+  float bound = bound_s[0];
+#pragma unroll
+  for (int w = 1; w < T / 64; ++w) bound = fmaxf(bound, bound_s[w]);
+  auto add = [&](double score, int flat) {   // (any order: it is ranked below)
+    const int at = atomicAdd(&n_s, 1);
+    score_s[at] = score, flat_s[at] = flat;
+  };
   if (self >= 0) {
     if (head > -INFINITY && (float)head >= bound) add(head, self);
   } else if (offset > -INFINITY) {
@@ -318,19 +313,26 @@ __global__ __launch_bounds__(256) void beam_pick_kernel(BeamSelect a, int parts,
     a.out_finished[row0 + slot] = done ? 1 : 0;
   };
 #pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const Pick one = list_s[i];
+  for (int i = threadIdx.x; i < n; i += T) {
+    const double score = score_s[i];
+    const int flat = flat_s[i];
     int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += before(list_s[j], one) ? 1 : 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += score_s[j] > score || (score_s[j] == score && flat_s[j] < flat) ? 1 : 0;
     if (rank < K) {
-      const int parent = one.flat / a.vocab;
-      const bool over = a.finished[row0 + parent] != 0;
-      const int token = over ? a.eos : one.flat - parent * a.vocab;
-      put(rank, one.score, parent, token, over || token == a.eos);
+      const int parent = flat / a.vocab;
+      const bool over = end_s[parent] != 0;
+      const int token = over ? a.eos : flat - parent * a.vocab;
+      put(rank, score, parent, token, over || token == a.eos);
     }
   }
   if ((int)threadIdx.x >= n && (int)threadIdx.x < K) put(threadIdx.x, -INFINITY, threadIdx.x, a.eos, true);   // too few candidates
+}
+
+int lanes_shift(int parts) {
+  int s = 0;
+  while (1 << s < parts) ++s;
+  return s;
 }
 
 // parts of a row: enough waves to fill the chip, at least a chunk each, and lists that pass 2 holds at one a thread
@@ -339,11 +341,19 @@ int beam_parts(int batch, int beams, int vocab) {
   int64_t n = (12288 + rows - 1) / rows;
   const int64_t chunks = (vocab + 64 * kLane - 1) / (64 * kLane);
   n = n < chunks ? n : chunks;
-  const int64_t most = kPicks / (beams * beams);
+  const int64_t most = picks_of(512) / (beams * beams);
   n = n < most ? n : most;
-  n = n < 256 / beams ? n : 256 / beams;
   n = n < kPartsMax ? n : kPartsMax;
-  return (int)(n < 1 ? 1 : n);
+  n = n < 1 ? 1 : n;
+  while ((beams << lanes_shift((int)n)) > 512) n = 1 << (lanes_shift((int)n) - 1);
+  return (int)n;
+}
+
+template <int KMAX>
+void launch_pick(const BeamSelect& a, int parts, const uint8_t* work, hipStream_t s) {
+  const int shift = lanes_shift(parts);
+  if (a.beams << shift <= 256 && a.beams * a.beams * parts <= picks_of(256)) MSH_LAUNCH((beam_pick_kernel<KMAX, 256>), dim3(a.batch), dim3(256), 0, s, a, parts, shift, work);
+  else MSH_LAUNCH((beam_pick_kernel<KMAX, 512>), dim3(a.batch), dim3(512), 0, s, a, parts, shift, work);
 }
 
 // ---- reordering ---------------------------------------------------------------------------------------------------------
@@ -478,9 +488,9 @@ void beam_select(const BeamSelect& a, Elem type, hipStream_t s) {
   if (type == Elem::f32) MSH_LAUNCH((beam_partial_kernel<Elem::f32>), grid, dim3(256), 0, s, a, parts, work);
   else if (type == Elem::bf16) MSH_LAUNCH((beam_partial_kernel<Elem::bf16>), grid, dim3(256), 0, s, a, parts, work);
   else MSH_LAUNCH((beam_partial_kernel<Elem::f16>), grid, dim3(256), 0, s, a, parts, work);
-  if (a.beams <= 4) MSH_LAUNCH(beam_pick_kernel<4>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
-  else if (a.beams <= 8) MSH_LAUNCH(beam_pick_kernel<8>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
-  else MSH_LAUNCH(beam_pick_kernel<16>, dim3(a.batch), dim3(256), 0, s, a, parts, work);
+  if (a.beams <= 4) launch_pick<4>(a, parts, work, s);
+  else if (a.beams <= 8) launch_pick<8>(a, parts, work, s);
+  else launch_pick<16>(a, parts, work, s);
 }
 
 void beam_reorder(const BeamState* states, int n_states, int batch, int beams, const int32_t* parents, const int32_t* lengths,

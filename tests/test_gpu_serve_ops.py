@@ -435,7 +435,8 @@ def check_select(logits, scores, finished, eos, sure=0.9, **layout):
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("batch, beams, vocab", [(1, 1, 1), (2, 3, 2), (1, 4, 512), (3, 2, 33), (5, 16, 17), (4, 5, 1000), (2, 8, 2049), (1, 4, 32768),
-                                                 (40, 3, 5003), (2, 16, 30001), (300, 2, 700), (1, 2, 150001)])
+                                                 (40, 3, 5003), (2, 16, 30001), (300, 2, 700), (1, 2, 150001), (1, 7, 193001), (2, 11, 90000),
+                                                 (1, 16, 70001), (1, 5, 140000), (3, 10, 50)])
 def test_select(dtype, batch, beams, vocab):
     rng = gen(batch * 7 + vocab)
     logits = dev((3 * rng.standard_normal((batch, beams, vocab))).astype(np.float32), TYPES[dtype])
@@ -461,6 +462,13 @@ def test_select_ties_go_to_the_lowest(dtype, beams):
         ids = list(range(5, vocab, 3))                       # of 40 ids, twelve: the next beam's follow
         assert got[2][0].tolist() == [ids[i % len(ids)] for i in range(beams)]
         assert got[1][0].tolist() == [i // len(ids) for i in range(beams)]
+
+
+@pytest.mark.parametrize("beams", [3, 8, 13])
+def test_select_ties_over_long_rows(beams):
+    """As many lists and candidates as the second pass can hold, all equal."""
+    got = check_select(torch.zeros((2, beams, 140000), device="cuda"), np.zeros((2, beams)), np.zeros((2, beams)), 5, sure=0.0)
+    assert got[1].tolist() == [[0] * beams] * 2 and got[2].tolist() == [list(range(beams))] * 2 and got[3][:, 5:6].all()
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
