@@ -331,7 +331,8 @@ MSH_EXPORT int64_t msh_host_biaser_bonuses(const int32_t* flat_tokens, const int
  * All pointers are device pointers of `device`; `stream` is a hipStream_t of that device (NULL: its default stream).  The calling
  * thread's current device is left as it was.  Calls enqueue and return: nothing is allocated, copied or waited for, no state is kept
  * between calls, so any number of threads and streams may call at once and every call may be captured into a graph -- with a
- * workspace of its own for each call that can run at the same time.  Results do not depend on what else runs (no atomics).
+ * workspace of its own for each call that can run at the same time.  Results do not depend on what else runs (no sum's order
+ * does).
  * Return 0 or a negative msh_status; msh_op_last_error() is the calling thread's message.
  * ------------------------------------------------------------------------------------------------- */
 enum msh_dtype { MSH_F32 = 0, MSH_BF16 = 1, MSH_F16 = 2 };
@@ -370,11 +371,11 @@ MSH_EXPORT int32_t msh_kv4_read(int32_t device, void* stream, const msh_kv4_cach
                                 void* v, int32_t dtype);
 
 /* out[r, h] = softmax(scale * q[r, h] . K) V over the cached tokens of row r's sequence; query head h reads cache head
- * h / (heads / cache.heads).  Sequence b has rows q_start[b] .. q_start[b + 1] - 1 (at most max_q of them; NULL: max_q rows each) and
- * kv_lens[b] tokens in the pages block_table[b][..].  causal: the rows are its LAST tokens, row i sees the tokens up to and including
+ * h / (heads / cache.heads).  Sequence b has rows q_start[b] .. q_start[b + 1] - 1 (at most max_q of them; NULL: max_q rows each;
+ * q_start must not decrease) and kv_lens[b] tokens in the pages block_table[b][..].  causal: the rows are its LAST tokens, row i sees the tokens up to and including
  * kv_lens[b] - n_rows + i, of these only the last `window` if window > 0; otherwise every row sees all.  A row that sees nothing gets
- * zeros and lse = -inf.  Tokens in a page that is not in the cache count as masked.  Rows of no sequence are left as they are; lse
- * [rows][heads] (nullable) is the natural logarithm of the sum of exponentials.  out has q's type.  Sums and the softmax are fp32;
+ * zeros and lse = -inf.  Tokens in a page that is not in the cache count as masked.  Rows of no sequence are left as they are; out
+ * may be q itself, or must not overlap it; lse [rows][heads] (nullable) is the natural logarithm of the sum of exponentials.  out has q's type.  Sums and the softmax are fp32;
  * bf16 outputs take p as two bf16 terms, fp32 ones as three.  The number of key ranges, and so the summation order, goes by the sizes
  * of the call (not by the lengths). */
 typedef struct msh_kv4_attention_args {
@@ -412,7 +413,7 @@ MSH_EXPORT int32_t msh_beam_select(int32_t device, void* stream, const void* log
  * each (outer o, entry b, beam k, inner i), at data + o * outer_stride + (b * beams + k) * beam_stride + i * inner_stride: a cache
  * [layers][entries * beams][heads][room][width] has outer = layers, inner = heads, row_bytes = width * size.  lengths: device int32, one
  * per entry (length_stride 1) or one for all (0), NULL: n_rows.  A parent that is no beam leaves its child as it is.  The states and
- * their rows must not overlap. */
+ * their rows must not overlap (rows that do, and an address given twice, are refused). */
 typedef struct msh_beam_state {
   void* data;
   int64_t outer, outer_stride, beam_stride, inner, inner_stride, row_bytes, n_rows; /* strides in bytes */

@@ -493,6 +493,21 @@ void beam_select(const BeamSelect& a, Elem type, hipStream_t s) {
   else launch_pick<16>(a, parts, work, s);
 }
 
+static int64_t piece_bytes(const BeamState& st) {
+  auto fits = [&](int64_t u) {
+    return (uintptr_t)st.data % u == 0 && (st.outer == 1 || st.outer_stride % u == 0) && st.beam_stride % u == 0 &&
+           (st.inner == 1 || st.inner_stride % u == 0);
+  };
+  return fits(16) ? 16 : fits(4) ? 4 : 1;
+}
+int64_t beam_reorder_groups(const BeamState* states, int n_states, int batch) {
+  int64_t n = 0;
+  for (int i = 0; i < n_states; ++i) {
+    const int64_t bytes = states[i].n_rows * states[i].row_bytes, slice = 256 * piece_bytes(states[i]);
+    n += states[i].outer * batch * states[i].inner * ((bytes + slice - 1) / slice);
+  }
+  return n;
+}
 void beam_reorder(const BeamState* states, int n_states, int batch, int beams, const int32_t* parents, const int32_t* lengths,
                   int length_stride, hipStream_t s) {
   BeamStates all{};
@@ -502,11 +517,7 @@ void beam_reorder(const BeamState* states, int n_states, int batch, int beams, c
     const BeamState& st = states[i];
     const int64_t bytes = st.n_rows * st.row_bytes;
     if (bytes == 0 || st.outer == 0 || st.inner == 0) continue;
-    auto fits = [&](int64_t u) {
-      return (uintptr_t)st.data % u == 0 && (st.outer == 1 || st.outer_stride % u == 0) && st.beam_stride % u == 0 &&
-             (st.inner == 1 || st.inner_stride % u == 0);
-    };
-    const int64_t unit = fits(16) ? 16 : fits(4) ? 4 : 1, slice = 256 * unit;
+    const int64_t unit = piece_bytes(st), slice = 256 * unit;
     all.s[n] = st;
     all.first[n] = (uint32_t)blocks;
     all.unit[n] = (int32_t)unit;

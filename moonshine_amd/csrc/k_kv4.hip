@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void page_plan_kernel(Plan p) {
   __syncthreads();
   first = red[0] + red[1] + red[2] + red[3];
   const int kept = pages_of(held - fresh, shift), need = pages_of(held, shift);
-  if (b == p.batch - 1 && threadIdx.x == 0) *p.used = (int32_t)(first + need - kept);
+  if (b == p.batch - 1 && threadIdx.x == 0) *p.used = (int32_t)min(first + need - kept, (int64_t)INT_MAX);
   int32_t* row = p.table + (int64_t)b * p.width;
   auto page_at = [&](int c) -> int32_t {   // (kept entries are read, the others written: by no other workgroup)
     if (c < kept) return row[c];

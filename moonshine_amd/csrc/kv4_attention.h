@@ -320,7 +320,7 @@ __device__ __forceinline__ void put_row(const Kv4Attention& a, int split, int64_
     if (first) p[DP] = top, p[DP + 1] = sum;
     return;
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = v[e] * inv;
@@ -339,7 +339,7 @@ __device__ __forceinline__ void put_row(const Kv4Attention& a, int split, int64_
     for (int e = 0; e < 8; ++e)
       if (d0 + e < a.cache.head_dim) o[e] = ElemOf<E>::put(x[e]);
   }
-  if (first && a.lse != nullptr) a.lse[row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
+  if (first && a.lse != nullptr) a.lse[row * a.heads + h] = sum != 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 // a wave's own rows
@@ -767,7 +767,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   float sum = lane < a.nsplit ? stat.y * f : 0.f;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   float4 v{0.f, 0.f, 0.f, 0.f};
   auto add = [&](int turn, const float4& x) {
     const int s = turn * groups + (has ? group : 0);
@@ -800,7 +800,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
       }
     }
   }
-  if (lane == 0 && a.lse != nullptr) a.lse[(int64_t)row * a.heads + h] = sum > 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
+  if (lane == 0 && a.lse != nullptr) a.lse[(int64_t)row * a.heads + h] = sum != 0.f ? (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f : -INFINITY;
 }
 
 template <int M, Elem E>

@@ -5,7 +5,9 @@
 
 #include <stdio.h>
 
+#include <algorithm>
 #include <string>
+#include <utility>
 
 #include "serve_kernels.h"
 
@@ -135,7 +137,7 @@ int32_t msh_kv4_write(int32_t device, void* stream, const msh_kv4_cache* cache, 
   return op_guarded([&] {
     const msh::Kv4Cache c = cache_of(cache);
     const msh::Elem t = elem(dtype);
-    need(rows >= 0 && rows <= kMost && rows * c.heads <= kMost * 8, "rows: too many for one launch");
+    need(rows >= 0 && rows < (1 << 26), "rows: 0 to 2^26 - 1");
     if (rows == 0) return;
     need(k && v && k_strides && v_strides && slots, "null pointer");
     DeviceScope scope(device);
@@ -149,7 +151,7 @@ int32_t msh_kv4_read(int32_t device, void* stream, const msh_kv4_cache* cache, c
   return op_guarded([&] {
     const msh::Kv4Cache c = cache_of(cache);
     const msh::Elem t = elem(dtype);
-    need(rows >= 0 && rows <= kMost && rows * c.heads <= kMost * 8, "rows: too many for one launch");
+    need(rows >= 0 && rows < (1 << 26), "rows: 0 to 2^26 - 1");
     if (rows == 0) return;
     need(k && v && slots, "null pointer");
     DeviceScope scope(device);
@@ -183,7 +185,7 @@ int32_t msh_kv4_attention(int32_t device, void* stream, const msh_kv4_attention_
 }
 
 static void select_sizes(int32_t batch, int32_t beams, int32_t vocab) {
-  need(batch >= 0 && batch <= (1 << 24), "batch: 0 to 2^24");
+  need(batch >= 0 && batch <= (1 << 21), "batch: 0 to 2^21");
   need(beams >= 1 && beams <= msh::kBeamMax, "beams: 1 to 16");
   need(vocab >= 1 && vocab <= (1 << 24), "vocab: 1 to 2^24");
 }
@@ -218,6 +220,19 @@ int32_t msh_beam_select(int32_t device, void* stream, const void* logits, int32_
   });
 }
 
+// no two of a state's (outer, entry and beam, inner) pieces of `bytes` share a byte: from the smallest stride up, each steps over what lies below
+static void apart(const msh_beam_state& x, int64_t bytes, int64_t rows) {
+  if (bytes == 0 || x.outer == 0 || x.inner == 0) return;
+  std::pair<int64_t, int64_t> by[3] = {{x.outer_stride, x.outer}, {x.beam_stride, rows}, {x.inner_stride, x.inner}};
+  std::sort(by, by + 3);
+  double extent = (double)bytes;
+  for (const auto& d : by) {
+    if (d.second == 1) continue;
+    need((double)d.first >= extent, "state: its rows overlap");
+    extent += (double)d.first * (double)(d.second - 1);
+  }
+}
+
 int32_t msh_beam_reorder(int32_t device, void* stream, const msh_beam_state* states, int32_t n_states, int32_t batch, int32_t beams,
                          const int32_t* parents, const int32_t* lengths, int32_t length_stride) {
   return op_guarded([&] {
@@ -228,7 +243,6 @@ int32_t msh_beam_reorder(int32_t device, void* stream, const msh_beam_state* sta
     if (batch == 0 || n_states == 0) return;
     need(parents != nullptr, "null pointer");
     msh::BeamState st[msh::kBeamStates];
-    int64_t blocks = 0;
     for (int i = 0; i < n_states; ++i) {
       const msh_beam_state& x = states[i];
       need(x.outer >= 0 && x.inner >= 0 && x.row_bytes >= 0 && x.n_rows >= 0 && x.outer <= kMost && x.inner <= kMost && x.row_bytes <= kMost &&
@@ -236,14 +250,12 @@ int32_t msh_beam_reorder(int32_t device, void* stream, const msh_beam_state* sta
       const int64_t bytes = x.row_bytes * x.n_rows;
       need(bytes <= ((int64_t)1 << 40), "state: a beam's rows are too large");
       need(x.outer == 0 || x.inner == 0 || bytes == 0 || x.data != nullptr, "null pointer");
-      need(beams == 1 || x.beam_stride >= bytes, "state: the rows of two beams overlap");
-      need(x.inner <= 1 || x.inner_stride >= bytes, "state: the rows of two inner entries overlap");
-      const double b = (double)x.outer * x.inner * batch * (double)(bytes / 256 + 1);
-      need(b < 2147483648.0, "state: too large for one launch");
-      blocks += (int64_t)b;
+      need((double)x.outer * x.inner * batch * (double)(bytes / 256 + 1) < 2147483648.0, "state: too large for one launch");
+      apart(x, bytes, (int64_t)batch * beams);
+      for (int j = 0; j < i; ++j) need(x.data != states[j].data || x.data == nullptr, "states: the same address twice");
       st[i] = msh::BeamState{x.data, x.outer, x.outer_stride, x.beam_stride, x.inner, x.inner_stride, x.row_bytes, x.n_rows};
     }
-    need(blocks < ((int64_t)1 << 31), "states: too large for one launch");
+    need(msh::beam_reorder_groups(st, n_states, batch) < (1 << 24), "states: too large for one launch");   // (a grid has 2^32 threads)
     DeviceScope scope(device);
     msh::beam_reorder(st, n_states, batch, beams, parents, lengths, length_stride, (hipStream_t)stream);
   });

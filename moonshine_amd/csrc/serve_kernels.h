@@ -99,6 +99,7 @@ struct BeamState {
   int64_t outer, outer_stride, beam_stride, inner, inner_stride, row_bytes, n_rows;
 };
 constexpr int kBeamStates = 4;
+int64_t beam_reorder_groups(const BeamState* states, int n_states, int batch);   // workgroups of the launch: below 2^24
 void beam_reorder(const BeamState* states, int n_states, int batch, int beams, const int32_t* parents, const int32_t* lengths,
                   int length_stride, hipStream_t s);
 

@@ -49,6 +49,12 @@ int64_t integer(PyObject* o, const char* name) {
   return v;
 }
 
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyFailed{};
+  return v != 0;
+}
+
 // the device that all tensors share, and torch's current stream there
 struct Place {
   int32_t device;
@@ -208,7 +214,7 @@ PyObject* kv4_attention(PyObject* const* a) {
     if (x.rows == 0) batch = 0, max_q = 1;
   }
   x.batch = small(batch, "batch"), x.max_q = small(max_q, "max_q");
-  x.causal = a[7] == Py_True ? 1 : a[7] == Py_False ? 0 : (int32_t)(integer(a[7], "causal") != 0);
+  x.causal = truth(a[7]) ? 1 : 0;
   x.window = small(integer(a[8], "window"), "window");
   if (a[6] == Py_None) {
     x.scale = (float)(1.0 / std::sqrt((double)q.size(2)));
@@ -223,11 +229,16 @@ PyObject* kv4_attention(PyObject* const* a) {
     p.same(out);
     if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || (out.stride(2) != 1 && q.size(2) > 1))
       refuse("out: q's shape and type, with a contiguous last dimension");
+    no_grad(out);
+    const int64_t rows = out.size(0), heads = out.size(1), width = out.size(2), r = out.stride(0), h = out.stride(1);
+    const bool by_row = (heads == 1 || h >= width) && (rows == 1 || r >= (heads - 1) * h + width);
+    const bool by_head = (rows == 1 || r >= width) && (heads == 1 || h >= (rows - 1) * r + width);
+    if (rows > 0 && !by_row && !by_head) refuse("out: its rows overlap");
   } else {
     out = make(p, q.sizes(), q.scalar_type());
   }
   at::Tensor lse;
-  const bool with_lse = a[9] == Py_True;
+  const bool with_lse = truth(a[9]);
   if (with_lse) lse = make(p, {x.rows, q.size(1)}, at::kFloat);
   x.q = q.data_ptr(), x.out = out.data_ptr(), x.lse = with_lse ? (float*)lse.data_ptr() : nullptr;
   x.q_row_stride = q.stride(0), x.q_head_stride = q.stride(1), x.out_row_stride = out.stride(0), x.out_head_stride = out.stride(1);

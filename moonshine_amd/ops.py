@@ -61,18 +61,16 @@ def kv4_cache(pages: int, heads: int, page_size: int, head_dim: int, device="cud
 def page_plan(block_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch.Tensor, row_start: torch.Tensor, rows: int,
               free_pages: torch.Tensor, page_size: int):
     """Extend ``block_table`` (int32 [batch, width], in place) to ``kv_lens`` tokens per request with pages from ``free_pages``,
-    and map the step's packed rows to slots.  ``new_lens[b]`` of the tokens are new and stand in rows ``row_start[b]``...
+    and map the step's packed rows to slots.  ``new_lens[b]`` of the tokens are new and stand in rows ``row_start[b]``... (not decreasing).
     Returns (slots int64 [rows], -1 for rows of no request; used int32 [1]: pages taken from ``free_pages``, which were too few
     if it exceeds their number -- the entries and slots that found no page are then -1)."""
     return _ops.page_plan(block_table, kv_lens, new_lens, row_start, rows, free_pages, page_size)
-
 
 
 def kv4_write(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Store rows of keys and values [rows, heads, head_dim] (fp32, bf16 or fp16, any strides) in their slots; a slot outside the
     cache (-1: padding) is skipped.  The slots of a call must differ.  NaN is stored as 0, infinities as the largest finite."""
     _ops.kv4_write(cache, k, v, slots)
-
 
 
 def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: torch.dtype = torch.bfloat16):
@@ -82,21 +80,19 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, dtype: tor
     return _ops.kv4_read(cache, slots, head_dim, _DTYPES[dtype])
 
 
-
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *,
                   q_start: torch.Tensor | None = None, max_q: int | None = None, scale: float | None = None, causal: bool = True,
                   window: int = 0, return_lse: bool = False, out: torch.Tensor | None = None):
     """Attention of packed query rows ``q`` [rows, heads, head_dim] over the cached tokens of their sequences.
 
-    Sequence b has the rows ``q_start[b]`` to ``q_start[b + 1] - 1``, at most ``max_q`` of them (``q_start`` None: rows / batch
-    each), and ``kv_lens[b]`` tokens in the pages ``block_table[b]``.  ``causal``: its rows are its last tokens, each sees what
+    Sequence b has the rows ``q_start[b]`` to ``q_start[b + 1] - 1``, at most ``max_q`` of them (``q_start``, not decreasing, int32 on
+    the GPU; None: rows / batch each), and ``kv_lens[b]`` tokens in the pages ``block_table[b]``.  ``causal``: its rows are its last tokens, each sees what
     stands up to itself, of that the last ``window`` tokens if window > 0; otherwise every row sees all tokens (a clip's
     encoder frames).  heads must be a multiple of the cache's: neighbouring query heads share one.  ``scale`` defaults to
     head_dim ** -0.5.  A row that sees nothing gives zeros and lse -inf; rows of no sequence are left as they are (in ``out``,
-    [rows, heads, head_dim] with a contiguous last dimension; uninitialised if none is given).
+    [rows, heads, head_dim] with a contiguous last dimension; uninitialised if none is given; it may be q itself).
     Returns out, or (out, lse fp32 [rows, heads])."""
     return _ops.kv4_attention(q, cache, block_table, kv_lens, q_start, max_q, scale, causal, window, return_lse, out)
-
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor, eos: int):
@@ -105,7 +101,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     Returns (scores, parents int32, tokens int32, finished) [batch, beams]: the best of score + log_softmax(logits), ties to the
     lowest beam * vocab + id; a finished beam stays as it is with the token ``eos`` (-1: no id ends a beam).  1 to 16 beams."""
     return _ops.beam_select(logits, scores, finished, eos)
-
 
 
 def beam_reorder(states, parents: torch.Tensor, lengths: torch.Tensor | None = None, *, batch_dims, row_dims) -> None:

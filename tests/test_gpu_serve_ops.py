@@ -289,6 +289,24 @@ def test_attention_chunks_with_pages_that_are_not_there():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("batch, rows, n", [(2, 1, 90), (2, 20, 90), (64, 70, 90), (1, 1, 5000)])
+def test_attention_into_its_own_queries_and_rows_of_nan(batch, rows, n):
+    """out may be q; a NaN query gives NaN (lse too) in its own row and in no other."""
+    cache = ops.kv4_cache(80, 8, 64, 64)
+    t = torch.arange(80 * 64, device="cuda")
+    ops.kv4_write(cache, dev(values(gen(6), (len(t), 8, 64))), dev(values(gen(7), (len(t), 8, 64))), t)
+    table = i32([[(b + j) % 80 for j in range(80)] for b in range(batch)])
+    q = dev(values(gen(8), (batch * rows, 8, 64)), torch.bfloat16)
+    lens = i32([n] * batch)
+    want, lse = ops.kv4_attention(q, cache, table, lens, max_q=rows, return_lse=1)
+    bad = q.clone()
+    bad[0, 3, 5] = float("nan")
+    got, got_lse = ops.kv4_attention(bad, cache, table, lens, max_q=rows, return_lse=True, out=bad)
+    assert got.data_ptr() == bad.data_ptr() and got[0, 3].isnan().all() and got_lse[0, 3].isnan()
+    got[0, 3], got_lse[0, 3] = want[0, 3], lse[0, 3]
+    assert torch.equal(got, want) and torch.equal(got_lse, lse)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_attention_sharp_and_flat_rows(dtype):
     """Scores of hundreds (one token takes all; the running maximum moves often) and of nothing."""
@@ -557,7 +575,7 @@ def test_reorder_several_states_at_once():
 def test_wrappers_refuse():
     z = lambda *s, t=torch.float32: torch.zeros(s, dtype=t, device="cuda")  # noqa: E731
     cache = ops.kv4_cache(2, 2, 32, 40)
-    slots, table, lens = z(3, t=torch.int64), z(1, 2, t=torch.int32), z(1, t=torch.int32)
+    slots, table, lens, scores = z(3, t=torch.int64), z(1, 2, t=torch.int32), z(1, t=torch.int32), z(2, 3, 4)
     bad = [
         lambda: ops.kv4_write(cache, z(3, 2, 40).requires_grad_(), z(3, 2, 40), slots),
         lambda: ops.kv4_write(cache, z(3, 2, 40, t=torch.float64), z(3, 2, 40, t=torch.float64), slots),
@@ -576,6 +594,9 @@ def test_wrappers_refuse():
         lambda: ops.kv4_attention(z(1, 2, 80)[:, :, ::2], cache, table, lens),
         lambda: ops.kv4_attention(z(1, 2, 40), cache, table, lens, out=z(1, 2, 40, t=torch.bfloat16)),
         lambda: ops.kv4_attention(z(1, 2, 40).requires_grad_(), cache, table, lens),
+        lambda: ops.kv4_attention(z(1, 2, 40), cache, table, lens, out=z(1, 2, 40).requires_grad_()),
+        lambda: ops.kv4_attention(z(1, 2, 40), cache, table, lens, out=z(1, 1, 40).expand(1, 2, 40)),
+        lambda: ops.kv4_attention(z(2, 2, 40), cache, table, lens, max_q=2, out=z(160).as_strided((2, 2, 40), (60, 40, 1))),
         lambda: ops.page_plan(table, lens, lens, lens, -1, lens, 32),
         lambda: ops.page_plan(table, lens, lens, lens, 1, lens, 31),
         lambda: ops.page_plan(table.long(), lens, lens, lens, 1, lens, 32),
@@ -588,6 +609,8 @@ def test_wrappers_refuse():
         lambda: ops.beam_reorder([z(2, 3, 4)], z(2, 3, t=torch.int32), batch_dims=[0], row_dims=[1]),
         lambda: ops.beam_reorder([z(1, 3, 4).expand(2, 3, 4)], z(2, 3, t=torch.int32), batch_dims=[0], row_dims=[2]),
         lambda: ops.beam_reorder([z(2, 3, 4)], z(2, 3, t=torch.int32), z(3, t=torch.int32), batch_dims=[0], row_dims=[2]),
+        lambda: ops.beam_reorder([z(1, 2, 3, 4).expand(5, 2, 3, 4)], z(2, 3, t=torch.int32), batch_dims=[1], row_dims=[3]),
+        lambda: ops.beam_reorder([scores, scores], z(2, 3, t=torch.int32), batch_dims=[0, 0], row_dims=[2, 2]),
         lambda: ops.beam_reorder([z(2, 3, 4)] * 5, z(2, 3, t=torch.int32), batch_dims=[0] * 5, row_dims=[2] * 5),
     ]
     for i, call in enumerate(bad):

@@ -32,7 +32,8 @@ def _attention(**change):
     (dict(max_q=0), "max_q"), (dict(table_width=0), "table_width"), (dict(table_width=1 << 26), "table_width"),
     (dict(causal=0, window=4), "window needs causal"), (dict(window=-1), "window"), (dict(scale=float("nan")), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(q=0), "null"), (dict(out=0), "null"), (dict(table=0), "null"), (dict(lens=0), "null"),
-    (dict(heads=65537), "heads"), (dict(batch=1 << 21, rows=1 << 21, heads=1024, kv_heads=1024), "too large"),
+    (dict(heads=65537), "heads"), (dict(batch=1 << 21, rows=1 << 21, heads=1024, kv_heads=1024), "too large"), (dict(batch=1 << 20, rows=1 << 20, heads=16, kv_heads=16), "too large"),
+    (dict(batch=1 << 30, rows=0, starts=FAKE, heads=1024, kv_heads=1024, max_q=1 << 24), "too large"),
 ])
 def test_attention_refuses(change, says):
     lib = load_library()
@@ -101,6 +102,16 @@ def test_plan_write_select_reorder_refuse():
                      (dict(row_bytes=-8), "sizes"), (dict(outer=1 << 20, inner=1 << 20, inner_stride=64), "too large")):
         rc, msg = reorder(**kw)
         assert rc == -3 and word in msg
+    for kw, word in ((dict(outer=2, outer_stride=64), "overlap"), (dict(outer=2, outer_stride=0), "overlap"), (dict(batch=2, beams=1, beam_stride=0), "overlap"),
+                     (dict(inner=4, inner_stride=-64), "overlap"), (dict(inner=3, inner_stride=64, beam_stride=128), "overlap"), (dict(n=2), "twice"),
+                     (dict(n=1, outer=1 << 24, outer_stride=128), "too large")):
+        rc, msg = reorder(**kw)
+        assert rc == -3 and word in msg, (kw, rc, msg)
+    for kw, word in ((dict(batch=1 << 22), "batch"), (dict(batch=(1 << 21) + 1, beams=1), "batch")):
+        rc, msg = select(**kw)
+        assert rc == -3 and word in msg
+    rc, msg = write(rows=1 << 26)
+    assert rc == -3 and "rows" in msg
     assert lib.msh_kv4_page_bytes(8, 64, 52) == 8 * 2 * 2176
     assert lib.msh_kv4_page_bytes(8, 64, 0) == -3
 
