@@ -1660,8 +1660,8 @@ void Engine::kv4_attend(DecodeGroup& g, int layer, hipStream_t s) {
   a.cache = kv4_cache_of(kv4_cache_.as<char>() + layer * kv4_layer_bytes(), kv4_pages_, cfg_.heads, dh);
   a.rows = g.M, a.heads = cfg_.heads, a.batch = g.M / g.beams, a.width = kv4_width_, a.max_q = g.beams;
   a.scale_log2 = 1.44269504088896341f / sqrtf((float)dh);
-  // (one kernel set for every call: the order of a clip's sums must not go by what shares its call)
-  a.nsplit = uniform_kernels_ ? 1 : kv4_attention_splits(a, Elem::f32);
+  a.fixed = uniform_kernels_;   // (one kernel set for every call: the order of a clip's sums must not go by what shares its call)
+  a.nsplit = kv4_attention_splits(a, Elem::f32);
   const size_t need = kv4_attention_part_floats(a, a.nsplit) * sizeof(float);
   if (need > g.kv4_part.cap) throw std::runtime_error("kv4_attend: workspace not reserved");
   a.part = g.kv4_part.as<float>();
@@ -2132,7 +2132,7 @@ int Engine::decode_beams(int forced_steps, int32_t* tokens_out, int32_t* counts_
   moved |= g.scalars.reserve(16 * sizeof(int32_t));
   moved |= g.scores.reserve((size_t)M * 2 * sizeof(float));               // scores, next scores
   moved |= g.beam_out.reserve((size_t)M * 2 * sizeof(int32_t));           // parents, ids
-  moved |= g.beam_work.reserve(beam_select_work_bytes(n, K, V));
+  moved |= g.beam_work.reserve(beam_select_work_bytes(n, K, V, uniform_kernels_));
   moved |= g.row_clips.reserve((size_t)M * sizeof(ClipMeta));
   if (kv_dtype_ == 2) moved |= g.kv4_part.reserve(kv4_part_bytes(M, K));
   if (moved) ++g.gen;
@@ -2147,7 +2147,7 @@ int Engine::decode_beams(int forced_steps, int32_t* tokens_out, int32_t* counts_
   BeamLoop loop{g.tokens.as<int32_t>(), g.scalars.as<int32_t>(), g.scores.as<float>(), g.scores.as<float>() + M, g.finished.as<uint8_t>(),
                 g.finished.as<uint8_t>() + M, g.beam_out.as<int32_t>(), g.beam_out.as<int32_t>() + M, dstride, K, n};
   const BeamSelect pick{g.logits.p, V, loop.scores, loop.finished, loop.next_scores, g.beam_out.as<int32_t>(), g.beam_out.as<int32_t>() + M,
-                        loop.next_finished, g.beam_work.p, n, K, V, forced ? -1 : cfg_.eos};
+                        loop.next_finished, g.beam_work.p, n, K, V, forced ? -1 : cfg_.eos, uniform_kernels_};
   const int64_t head = (int64_t)Smax_ * dh * sizeof(bf16_t);
   const BeamState states[3] = {
       {g.cacheK.p, L, (int64_t)M * Hh * head, Hh * head, Hh, head, (int64_t)(dh * sizeof(bf16_t)), Smax_},

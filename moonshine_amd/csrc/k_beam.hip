@@ -336,8 +336,9 @@ int lanes_shift(int parts) {
 }
 
 // parts of a row: enough waves to fill the chip, at least a chunk each, and lists that pass 2 holds at one a thread
-int beam_parts(int batch, int beams, int vocab) {
-  const int64_t rows = (int64_t)batch * beams;
+// (fixed: as for one entry, whatever the batch is)
+int beam_parts(int batch, int beams, int vocab, bool fixed) {
+  const int64_t rows = (int64_t)(fixed ? 1 : batch) * beams;
   int64_t n = (12288 + rows - 1) / rows;
   const int64_t chunks = (vocab + 64 * kLane - 1) / (64 * kLane);
   n = n < chunks ? n : chunks;
@@ -477,12 +478,12 @@ void beam_advance(const BeamLoop& l, const ClipMeta* row_clips, const float* emb
   MSH_LAUNCH(beam_tick_kernel, dim3(1), dim3(1), 0, s, l.pos);
 }
 
-size_t beam_select_work_bytes(int batch, int beams, int vocab) {
-  return (size_t)batch * beams * beam_parts(batch, beams, vocab) * part_bytes(beams);
+size_t beam_select_work_bytes(int batch, int beams, int vocab, bool fixed) {
+  return (size_t)batch * beams * beam_parts(batch, beams, vocab, fixed) * part_bytes(beams);
 }
 
 void beam_select(const BeamSelect& a, Elem type, hipStream_t s) {
-  const int parts = beam_parts(a.batch, a.beams, a.vocab);
+  const int parts = beam_parts(a.batch, a.beams, a.vocab, a.fixed);
   const dim3 grid((unsigned)(((int64_t)a.batch * a.beams * parts + 3) / 4));
   uint8_t* work = static_cast<uint8_t*>(a.work);
   if (type == Elem::f32) MSH_LAUNCH((beam_partial_kernel<Elem::f32>), grid, dim3(256), 0, s, a, parts, work);

@@ -331,10 +331,11 @@ void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 //   23.6 / 17.1 / 15.3; 2048 tokens: 1280 units 55 / 62 / 85, 4096 units 191 / 181 / 184).
 Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads), pairs = (int64_t)a.batch * a.cache.heads;
-  if (rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
+  if (!a.fixed && rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
   if (rows > 16 && !(type == Elem::f32 && a.cache.head_dim > 96)) return Kv4Shape{2, 4, false};
   const int64_t units = pairs * ((rows + 15) / 16), room = (int64_t)a.width << a.cache.page_shift;
   const bool brief = room <= 1024;
+  if (a.fixed) return Kv4Shape{1, 4, false};
   return Kv4Shape{1, units >= (brief ? 2560 : 4096) ? 1 : units >= (brief ? 1024 : 2048) ? 2 : 4, false};
 }
 
@@ -348,7 +349,7 @@ Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
 // 485 to 1000 queries: 529 against 617; all of 8192: 771 against 752; at 2048 tokens the join would cost a quarter: 260 against 207).
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   const Kv4Shape shape = kv4_attention_shape(a, type);
-  if (shape.kw != 4 || a.rows * a.heads >= (1 << 26)) return 1;   // (a grid has 2^32 threads)
+  if (a.fixed || shape.kw != 4 || a.rows * a.heads >= (1 << 26)) return 1;   // (a grid has 2^32 threads)
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
   const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + shape.rows() - 1) / shape.rows());
   const int64_t room = (int64_t)a.width << a.cache.page_shift;

@@ -63,6 +63,7 @@ struct Kv4Attention {
   float scale_log2;           // softmax scale * log2(e)
   uint16_t* fm;               // not null: the engine's decode path takes the output as bf16, fragment-major [rows16][heads * head_dim]
                               // (kernels.h fm16), instead of `out`
+  bool fixed;                 // the order of a row's sums goes by nothing that its sequence does not bring along (uniform kernels)
 };
 constexpr int kPartPad = 4;       // a range's row: 32 m floats, maximum, sum, two unused
 // tile of a wave (16 * rt rows) and waves that share it, or the form for chunks of prompts; see kv4_attention.h
@@ -87,9 +88,10 @@ struct BeamSelect {
   uint8_t* out_finished;
   void* work;
   int32_t batch, beams, vocab, eos;
+  bool fixed = false;         // as in Kv4Attention
 };
 constexpr int kBeamMax = 16;
-size_t beam_select_work_bytes(int batch, int beams, int vocab);
+size_t beam_select_work_bytes(int batch, int beams, int vocab, bool fixed = false);
 void beam_select(const BeamSelect& a, Elem type, hipStream_t s);
 
 // byte strides; segment (o, b, k, i) starts at data + o * outer_stride + (b * beams + k) * beam_stride + i * inner_stride and holds

@@ -235,6 +235,30 @@ def test_beams_of_real_shapes_in_flight_and_profiled(tmp_path_factory, kv_dtype,
     e.close()
 
 
+@pytest.mark.parametrize("beams", [1, 3])
+def test_uniform_kernels_give_a_clip_the_same_bits_in_any_batch(tmp_path_factory, beams):
+    """mxfp4 under uniform kernels: a clip alone, and in a batch large enough and with a clip long enough that the attention would take
+    another form by itself."""
+    e, w, cfg = tp._engine(tmp_path_factory, "tiny", 0)
+    e.set_uniform_kernels(True)
+    e.set_kv_dtype("mxfp4")
+    clips = [make_audio(300 + i, 8000 + 512 * (i % 7)) for i in range(150)]
+    clips[140] = make_audio(9, 16000 * 24)
+    if beams == 1:
+        e.encode(clips)
+        _, all_logits = e.decode(forced_steps=3, want_logits=3)
+        for c in (0, 77, 149):
+            e.encode([clips[c]])
+            _, logits = e.decode(forced_steps=3, want_logits=3)
+            assert np.array_equal(logits[:, 0], all_logits[:, c])
+    else:
+        e.set_beam_width(beams)
+        together = e.transcribe_tokens(clips)
+        for c in (0, 77, 140, 149):
+            assert e.transcribe_tokens([clips[c]]) == [together[c]]
+    e.close()
+
+
 def test_transcriber_options(tmp_path_factory):
     """kv_dtype = mxfp4, beam_width and length_penalty through the C API: the text is that of the engine's own ids."""
     d = str(tmp_path_factory.mktemp("tiny_model"))
