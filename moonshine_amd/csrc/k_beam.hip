@@ -360,9 +360,9 @@ void launch_pick(const BeamSelect& a, int parts, const uint8_t* work, hipStream_
 // ---- reordering ---------------------------------------------------------------------------------------------------------
 // state[b, k, :len_b] <- state[b, parent[b, k], :len_b] in place.  A thread owns one piece (16 bytes) of all beams of (outer, b, inner): it
 // loads what its beams' parents have there, then stores -- no thread reads what another writes, whatever the parents are, and a beam
-// that continues itself is neither read nor written.  One piece a thread: several in turn
-// measured slower (four: 758 us instead of the figure below), since a workgroup's time is the latency of its chain of loads.  Bound by HBM
-// bandwidth.
+// that continues itself is neither read nor written.  One piece a thread: several in turn measured slower (four: 758 us instead of 238), since a
+// workgroup's time is the latency of its chain of loads.  Bound by HBM bandwidth: 8 layers of 32 entries x 8 beams x 8 heads, up to 447 rows of 52 bf16
+// keys and values (1.1 GB): 238 us, 4.6 TB/s; one clip's four beams after 33 steps: 7.3 us.
 struct BeamStates {
   BeamState s[kBeamStates];
   uint32_t first[kBeamStates];      // first workgroup of each state

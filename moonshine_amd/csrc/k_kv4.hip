@@ -9,7 +9,7 @@ namespace {
 // kept_b + i of request b becomes free[first_b + i], and the row at place p of request b the slot table[b][p / P] * P + p mod P.
 // One launch, one workgroup per request: each adds up the lengths of the requests before it for itself (8 bytes each, out of L2) instead of
 // waiting for a scan of its own launch, and clears the rows between its own and the next request's.  A few bytes per request: bound by
-// launch and memory latency.
+// launch and memory latency.  5 requests 2.9 us, 1999 with up to 16000 tokens each 6.2 us.
 struct Plan {
   int32_t* table;
   const int32_t *kv_lens, *new_lens, *row_start, *free_pages;
@@ -96,8 +96,9 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float scale) {
 // A workgroup: 4 rows x 16 (head, group) pairs x 4 quarters, a thread 8 elements of a key and of a value; its reads of a row are contiguous
 // over the heads.  Where four neighbouring rows are the four tokens of one aligned run of slots -- every prompt -- their lanes
 // exchange the value bytes (16 neighbouring lanes hold 4 tokens x 4 quarters) and store one dword of four tokens each instead of four
-// bytes.  One (head, group) a thread: a loop over the groups measured slower (its loads wait for one another).  Bound by HBM
-// bandwidth; single tokens by latency.
+// bytes.  One (head, group) a thread: a loop over the groups measured slower (its loads wait for one another).
+// 53120 bf16 rows of 8 heads of 52 (117 MB): 33 us, 3.5 TB/s, by the vector unit (two thirds busy: scales, codes, the exchange) beside HBM; reading
+// them back 24 us, 4.9 TB/s, what a copy reaches.  61 rows of 8 heads of 128: 3.5 us each, a launch.
 __device__ __forceinline__ uint32_t lanes_rotate4(uint32_t x) {   // from the lane 4 below within the 16, cyclically
   return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x124 /* row_ror:4 */, 0xf, 0xf, false);
 }
@@ -327,8 +328,8 @@ void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 // * 17 rows and more: tiles of 32 (32 sequences of 2048, 64 rows: 38 against 49 by tiles of 16), but for 32-bit rows of more than 96, which spill
 //   (64 rows: 70 by tiles of 16 against 76, 256 rows 246 against 294).
 // * tiles of 16: all four waves of a workgroup share a tile as long as there are too few to fill the chip without, then two, then none -- a wave's beginning
-//   and end cost as much as three blocks, so sooner for short tables (units, KW 4 / 2 / 1; 100 tokens: 1024 units 9.9 / 8.0 / 8.2, 3072 units
-//   23.6 / 17.1 / 15.3; 2048 tokens: 1280 units 55 / 62 / 85, 4096 units 191 / 181 / 184).
+//   and end cost as much as three blocks, so sooner for short tables (units, KW 4 / 2 / 1; 100 tokens: 1024 units 9.9 / 8.0 / 8.2, 4096 units
+//   31 / 22 / 20; 2048 tokens: 1280 units 55 / 62 / 85, 4096 units 191 / 181 / 184).
 Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads), pairs = (int64_t)a.batch * a.cache.heads;
   if (!a.fixed && rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
