@@ -143,8 +143,8 @@ def build_ops(force: bool = False) -> str:
     root = os.path.dirname(torch.__file__)
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{root}/include",
-           f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}", src, "-o", LIB_OPS,
-           f"-L{LIBDIR}", "-l:libmoonshine.so", f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
+           f"-I{root}/include/torch/csrc/api/include", "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{sysconfig.get_paths()['include']}", src, "-o", LIB_OPS,
+           f"-L{LIBDIR}", "-l:libmoonshine.so", f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10_hip", "-lc10", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")

@@ -4,11 +4,16 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
+#include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <stdexcept>
+#include <optional>
 #include <string>
 
 #include "moonshine_hip.h"
@@ -16,7 +21,6 @@
 namespace {
 
 PyObject* g_error = nullptr;    // MshError(code, message)
-PyObject* g_stream = nullptr;   // device index -> raw stream
 
 struct Refused {
   int code;
@@ -55,22 +59,18 @@ bool truth(PyObject* o) {
   return v != 0;
 }
 
-// the device that all tensors share, and torch's current stream there
+// the device that all tensors share, current for the call's allocations, and torch's current stream there
 struct Place {
   int32_t device;
   void* stream;
   c10::Device where;
+  c10::OptionalDeviceGuard guard;
 
   explicit Place(const at::Tensor& first) : device(0), stream(nullptr), where(first.device()) {
     if (!where.is_cuda()) refuse("tensors must be on the GPU, not on " + where.str() + ": there is no CPU fallback");
+    guard.reset_device(where);
     device = where.index();
-    PyObject* i = PyLong_FromLong(device);
-    PyObject* s = i ? PyObject_CallOneArg(g_stream, i) : nullptr;
-    Py_XDECREF(i);
-    if (s == nullptr) throw PyFailed{};
-    stream = PyLong_AsVoidPtr(s);
-    Py_DECREF(s);
-    if (PyErr_Occurred()) throw PyFailed{};
+    stream = (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(where.index()).stream();
   }
   const Place& same(const at::Tensor& t) const {
     if (t.device() != where) refuse("tensors on " + where.str() + " and " + t.device().str() + ": one call, one device");
@@ -102,7 +102,11 @@ void* array(const at::Tensor& t, const char* name, at::ScalarType type, at::IntA
   return t.data_ptr();
 }
 
-at::Tensor make(const Place& p, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, at::TensorOptions().dtype(type).device(p.where)); }
+// Outputs and workspaces come from torch's allocator without the dispatcher, which takes longer than the allocation (0.5 us each of a call's 5 to 10).
+c10::Allocator* allocator() { return c10::hip::HIPCachingAllocatorMasqueradingAsCUDA::get(); }
+at::Tensor make(const Place&, at::IntArrayRef shape, at::ScalarType type) {
+  return at::detail::empty_generic(shape, allocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
 
 msh_kv4_cache cache_of(const at::Tensor& t, int64_t head_dim) {
   if (t.scalar_type() != at::kByte || t.dim() != 4 || !t.is_contiguous())
@@ -243,9 +247,8 @@ PyObject* kv4_attention(PyObject* const* a) {
   x.q = q.data_ptr(), x.out = out.data_ptr(), x.lse = with_lse ? (float*)lse.data_ptr() : nullptr;
   x.q_row_stride = q.stride(0), x.q_head_stride = q.stride(1), x.out_row_stride = out.stride(0), x.out_head_stride = out.stride(1);
   const int64_t size = check(msh_kv4_attention_workspace(&x));
-  at::Tensor work;
-  if (size > 0) work = make(p, {size}, at::kByte);
-  check(msh_kv4_attention(p.device, p.stream, &x, size > 0 ? work.data_ptr() : nullptr, size));
+  const c10::DataPtr work = size > 0 ? allocator()->allocate((size_t)size) : c10::DataPtr();
+  check(msh_kv4_attention(p.device, p.stream, &x, work.get(), size));
   if (with_lse) return wrap({out, lse});
   return THPVariable_Wrap(out);
 }
@@ -269,10 +272,11 @@ PyObject* beam_select(PyObject* const* a) {
   auto* fp = (const uint8_t*)array(finished, "finished", flag, {batch, beams});
   const int64_t size = check(msh_beam_select_workspace(small(batch, "batch"), small(beams, "beams"), small(vocab, "vocab")));
   at::Tensor next = make(p, {batch, beams}, at::kFloat), parents = make(p, {batch, beams}, at::kInt), tokens = make(p, {batch, beams}, at::kInt),
-             ended = make(p, {batch, beams}, flag), work = make(p, {size}, at::kByte);
+             ended = make(p, {batch, beams}, flag);
+  const c10::DataPtr work = allocator()->allocate((size_t)size);
   check(msh_beam_select(p.device, p.stream, logits.data_ptr(), type, row, (int32_t)batch, (int32_t)beams, (int32_t)vocab, sp, fp, small(eos, "eos"),
                         (float*)next.data_ptr(), (int32_t*)parents.data_ptr(), (int32_t*)tokens.data_ptr(), (uint8_t*)ended.data_ptr(),
-                        work.data_ptr(), size));
+                        work.get(), size));
   return wrap({next, parents, tokens, ended});
 }
 
@@ -352,13 +356,12 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* set_up(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 2) {
-    PyErr_SetString(PyExc_TypeError, "set_up(error class, stream function)");
+  if (n != 1) {
+    PyErr_SetString(PyExc_TypeError, "set_up(error class)");
     return nullptr;
   }
   Py_INCREF(args[0]);
-  Py_INCREF(args[1]);
-  g_error = args[0], g_stream = args[1];
+  g_error = args[0];
   Py_RETURN_NONE;
 }
 

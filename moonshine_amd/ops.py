@@ -39,7 +39,7 @@ def _load():
     spec = importlib.util.spec_from_file_location("msh_torch_ops", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
-    module.set_up(MshError, torch._C._cuda_getCurrentRawStream)
+    module.set_up(MshError)
     return module
 
 
