@@ -322,30 +322,34 @@ void kv4_attention_f32(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_bf16(const Kv4Attention& a, hipStream_t s);
 void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 
-// Which form, by the rows of one key / value head and the work there is (times of 32 query over 8 key / value heads of 128, bf16, in us):
+// Which form, by the rows of one key / value head and the work there is (times in us; 32 query over 8 key / value heads of 128, bf16, unless it says otherwise):
 // * more than 64 rows: the form for chunks once its units of 128 rows fill the chip's 512 places (2048 tokens: 2 x 1024 queries 112 against 120 by
 //   tiles of 32, 64 sequences of 512 with 128 queries each 133 against 202; half as many units: 1 x 1024 queries 80 against 70).
-// * 17 rows and more: tiles of 32 (32 sequences of 2048, 64 rows: 38 against 49 by tiles of 16), but for 32-bit rows of more than 96, which spill
-//   (64 rows: 70 by tiles of 16 against 76, 256 rows 246 against 294).
-// * tiles of 16: all four waves of a workgroup share a tile as long as there are too few to fill the chip without, then two, then none -- a wave's beginning
-//   and end cost as much as three blocks, so sooner for short tables (units, KW 4 / 2 / 1; 100 tokens: 1024 units 9.9 / 8.0 / 8.2, 4096 units
-//   31 / 22 / 20; 2048 tokens: 1280 units 55 / 62 / 85, 4096 units 191 / 181 / 184).
+// * tiles of 32 once tiles of 16, four waves each, take more than half the places for waves (32 sequences of 2048, 20 rows: 27 against 29, 64 rows: 38 against
+//   49; fp32, 4 heads of 64, 32 rows, 256 units of 16: 12.7 against 8.6) -- but not for fp32 rows of more than 64, which spill (64 rows: 70 by tiles of
+//   16 against 76; 3 x 8 rows over 4 heads of 96, 128 sequences of 2000: 56 against 64).
+// * tiles of 16: all four waves of a workgroup share a tile as long as there are too few to fill the chip's places for waves (1024 SIMDs) without,
+//   then two, then none -- a wave's beginning and end cost as much as three blocks, so sooner for short tables and later for long ones (units, KW 4 / 2 / 1; fp32, two
+//   places a SIMD, 10 tokens: 512 units 8.9 / 7.4 / 7.6, 1024 units 15 / 9.1 / 7.7; three places, 415 tokens: 1024 units 15.8 / 14.4 / 16.6, 2048
+//   units 27 / 24 / 24; 2048 tokens: 1280 units 55 / 62 / 85, 1536 units 67 / 67 / 89, 4096 units 191 / 181 / 184).
 Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
+  const int groups = kv4_groups(a.cache.head_dim);
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads), pairs = (int64_t)a.batch * a.cache.heads;
-  if (!a.fixed && rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
-  if (rows > 16 && !(type == Elem::f32 && a.cache.head_dim > 96)) return Kv4Shape{2, 4, false};
   const int64_t units = pairs * ((rows + 15) / 16), room = (int64_t)a.width << a.cache.page_shift;
-  const bool brief = room <= 1024;
+  const int64_t places = 1024 * kv4_attention_waves(groups, type == Elem::f32);
   if (a.fixed) return Kv4Shape{1, 4, false};
-  return Kv4Shape{1, units >= (brief ? 2560 : 4096) ? 1 : units >= (brief ? 1024 : 2048) ? 2 : 4, false};
+  if (rows > 64 && pairs * ((rows + 127) / 128) >= 512) return Kv4Shape{2, 4, true};
+  if (rows > 16 && units * 8 > places && !(type == Elem::f32 && groups > 2)) return Kv4Shape{2, 4, false};
+  const int64_t ample = room <= 128 ? places / 2 : room <= 1024 ? places : places * 2;
+  return Kv4Shape{1, units * 4 <= ample ? 4 : units * 2 <= ample ? 2 : 1, false};
 }
 
 // Key ranges, joined by a second launch (4 to 40 us, by the rows).  The lengths live on the device; the host knows the table's room only.  A
 // range is a share of each sequence's own length, so a short sequence in a wide table costs empty ranges and nothing else.
 // Few units: as many ranges as fill the chip, none of them shorter than pays for its share of the join (single tokens, units x tokens, ranges 1 / 2 /
 // 4 / 8 / 16 / 32: 8 x 1024: 11 / 10 / 9.1 / 8.5 / 9.0 / 10; 64 x 4096: 29 / 20 / 15 / 14 / 17 / 24; 128 x 16384: 107 / 61 / 51 / 49 / 52 / 62, but with
-// lengths between 1500 and 16383 161 at 2, 116 at 8 and 106 at 16; 512 x 4096: 47 / 49 / 52 / 59; 32-row tiles: 32 x 8192: 73 / 44 / 29 / 22 / 26 / 34;
-// 256 x 2048: 27 / 32).  Below 1024 tokens one (8 units x 600: 8.4 / 9.7).
+// lengths between 12001 and 40000 161 at 2, 116 at 8 and 106 at 16; 512 x 4096: 47 / 49 / 52 / 59; fp32 512 x 2048 32 / 40; 32-row tiles: 32 x 8192: 73 /
+// 44 / 29 / 22 / 26 / 34; 256 x 2048: 27 / 32).  Below 1024 tokens one (8 units x 600: 8.4 / 9.7).
 // Chunks: two ranges where units are few enough for long and short sequences to leave places empty at the end (4 sequences of 2500 to 8191 tokens,
 // 485 to 1000 queries: 529 against 617; all of 8192: 771 against 752; at 2048 tokens the join would cost a quarter: 260 against 207).
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
@@ -356,8 +360,9 @@ int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   const int64_t room = (int64_t)a.width << a.cache.page_shift;
   if (shape.chunk) return units < 1536 && room >= 8192 ? 2 : 1;
   if (room < 1024) return 1;
-  const int64_t wanted = shape.rt == 2 ? 512 : room < 16384 ? 1024 : 2048;
-  const int64_t least = units <= 32 ? 256 : (units <= 128 ? 512 : 1024) * shape.rt;
+  const int64_t places = shape.rt == 2 ? 512 : 256 * kv4_attention_waves(kv4_groups(a.cache.head_dim), type == Elem::f32);   // for workgroups
+  const int64_t wanted = room < 16384 ? places : places * 5 / 2;
+  const int64_t least = units <= 32 ? 256 : (units <= 128 ? 512 : 2048) * shape.rt;
   int64_t n = wanted / units;
   n = n < room / least ? n : room / least;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);

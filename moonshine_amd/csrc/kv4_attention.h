@@ -369,8 +369,8 @@ __device__ __forceinline__ void put_walk(const Kv4Attention& a, int split, const
 // waves per SIMD: left alone the compiler spends the registers of two or three waves on one; asked for more it spills
 template <int M, Elem E, int RT>
 constexpr int waves_wanted() {
-  if (RT == 1) return M <= 2 ? 4 : M <= 4 && E != Elem::f32 ? 3 : 2;
-  return M <= 2 ? (E == Elem::bf16 ? 3 : 2) : M <= 4 && E != Elem::f32 ? 2 : 1;
+  if (RT == 1) return kv4_attention_waves(M, E == Elem::f32);
+  return M <= 2 ? (E == Elem::bf16 ? 3 : 2) : M <= 4 ? 2 : 1;
 }
 template <int M, Elem E, int RT, int KW>
 __global__ __launch_bounds__(256, (waves_wanted<M, E, RT>())) void kv4_attention_kernel(Kv4Attention a) {
@@ -830,7 +830,7 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
     if (shape.rt == 1 && shape.kw == 4) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 4>), grid, dim3(256), 0, s, a);
     else if (shape.rt == 1 && shape.kw == 2) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 2>), grid, dim3(256), 0, s, a);
     else if (shape.rt == 1) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 1>), grid, dim3(256), 0, s, a);
-    else MSH_LAUNCH((kv4_attention_kernel<M, E, 2, 4>), grid, dim3(256), 0, s, a);
+    else if constexpr (M <= 2 || E != Elem::f32) MSH_LAUNCH((kv4_attention_kernel<M, E, 2, 4>), grid, dim3(256), 0, s, a);   // (kv4_attention_shape())
   }
   const dim3 rows4((unsigned)((a.rows * a.heads + 3) / 4));
   if (a.nsplit > 1 && a.nsplit <= 64 / (8 * M)) MSH_LAUNCH((kv4_join_kernel<E, 1>), rows4, dim3(256), 0, s, a, 32 * M);

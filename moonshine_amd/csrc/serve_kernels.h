@@ -66,6 +66,8 @@ struct Kv4Attention {
   bool fixed;                 // the order of a row's sums goes by nothing that its sequence does not bring along (uniform kernels)
 };
 constexpr int kPartPad = 4;       // a range's row: 32 m floats, maximum, sum, two unused
+// waves per SIMD that the attention's registers allow (tiles of 16 rows)
+constexpr int kv4_attention_waves(int groups, bool f32) { return groups <= 2 ? 4 : groups <= 4 && !f32 ? 3 : 2; }
 // tile of a wave (16 * rt rows) and waves that share it, or the form for chunks of prompts; see kv4_attention.h
 struct Kv4Shape {
   int rt, kw;

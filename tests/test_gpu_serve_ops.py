@@ -271,6 +271,32 @@ def test_attention_batches_of_long_chunks(dtype, window):
     check_attention(dtype, 8, 8, 64, 64, [8200, 100, 0, 33] + [40] * 60, [70, 70, 3, 65] + [7] + [0] * 59, window=window, seed=15)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [52, 96, 128, 224, 256])
+@pytest.mark.parametrize("batch", [60, 110, 300])
+def test_attention_single_tokens_of_large_batches(dtype, width, batch):
+    """Sequences enough that four, two or one wave take a tile, in short tables and longer ones; most have no tokens."""
+    lengths = [33, 0, 120, 1, 64] + [0] * (batch - 7) + [95, 32]
+    check_attention(dtype, 8, 8, width, 32, lengths, [1] * batch, uniform=True, seed=16)
+    lengths[7] = 300
+    check_attention(dtype, 16, 8, width, 64, lengths, [1] * batch, seed=17)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [36, 64, 80, 128, 192, 256])
+@pytest.mark.parametrize("causal, window", [(True, 0), (False, 0), (True, 37)])
+def test_attention_drafts_of_large_batches(dtype, width, causal, window):
+    """The same with several rows a sequence: tiles of 32."""
+    counts, lengths = [40, 0, 17, 1, 64, 33] + [0] * 60 + [2, 50], [100, 64, 150, 203, 33, 1] + [0] * 60 + [97, 0]
+    check_attention(dtype, 8, 8, width, 32, lengths, counts, causal, window, seed=18)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_drafts_over_a_long_cache(dtype):
+    """Tiles of 32 and key ranges."""
+    check_attention(dtype, 8, 8, 52, 64, [16500, 40, 0, 300] + [1] * 40, [33, 20, 1, 2] + [1] + [0] * 39, seed=19)
+
+
 def test_attention_chunks_with_pages_that_are_not_there():
     """A page outside the cache counts as absent in every form: its tokens get no weight."""
     batch, rows, n = 64, 70, 160
