@@ -97,8 +97,8 @@ __device__ __forceinline__ uint32_t codes8(const float* x, float scale) {
 // over the heads.  Where four neighbouring rows are the four tokens of one aligned run of slots -- every prompt -- their lanes
 // exchange the value bytes (16 neighbouring lanes hold 4 tokens x 4 quarters) and store one dword of four tokens each instead of four
 // bytes.  One (head, group) a thread: a loop over the groups measured slower (its loads wait for one another).
-// 53120 bf16 rows of 8 heads of 52 (117 MB): 33 us, 3.5 TB/s, by the vector unit (two thirds busy: scales, codes, the exchange) beside HBM; reading
-// them back 24 us, 4.9 TB/s, what a copy reaches.  61 rows of 8 heads of 128: 3.5 us each, a launch.
+// 53120 bf16 rows of 8 heads of 52 (117 MB): 28 us, 4.2 TB/s, by the vector unit (scales, codes, the exchange; with floats made of the 16-bit elements
+// first it was 33) beside HBM; reading them back 24 us, 4.9 TB/s, what a copy reaches.  61 rows of 8 heads of 128: 3.5 us each, a launch.
 __device__ __forceinline__ uint32_t lanes_rotate4(uint32_t x) {   // from the lane 4 below within the 16, cyclically
   return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x124 /* row_ror:4 */, 0xf, 0xf, false);
 }
@@ -153,6 +153,70 @@ __device__ __forceinline__ uint8_t* item_block(const Kv4Cache& c, const Item& it
   return c.data + (((page * c.heads + it.h) << (c.page_shift - 5)) + (place >> 5)) * kv4_block_bytes(m);
 }
 
+// eight elements of a thread as they are read: floats, or 16-bit elements in pairs, whose largest magnitude and codes take half the instructions
+template <Elem E>
+struct Eight {
+  uint32_t w[4];
+  __device__ __forceinline__ void load4(const void* p, int half) {
+    const uint2 u = *static_cast<const uint2*>(p);
+    w[2 * half] = u.x, w[2 * half + 1] = u.y;
+  }
+  __device__ __forceinline__ void set(int e, uint16_t v) { w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | (uint32_t)v << 16 : v; }
+  __device__ __forceinline__ void clear_from(int n) {   // elements n and behind (n a constant after unrolling, or the row's end)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 2 * i >= n ? 0u : 2 * i + 1 >= n ? w[i] & 0xffffu : w[i];
+  }
+  __device__ __forceinline__ uint32_t abs_max() const {   // as the bits of a float
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    const uint32_t a = max((uint32_t)m[0], (uint32_t)m[1]);
+    if constexpr (E == Elem::bf16) return a << 16;
+    return __float_as_uint(ElemOf<E>::get((typename ElemOf<E>::T)a));
+  }
+  __device__ __forceinline__ void floats(float* x) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t v = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+      x[e] = ElemOf<E>::get((typename ElemOf<E>::T)v);
+    }
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const {
+    uint32_t r = 0;
+    if constexpr (E == Elem::bf16) {
+      typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[0]), scale, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
+    } else {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w[0]), scale, 0);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w[1]), scale, 1);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w[2]), scale, 2);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, w[3]), scale, 3);
+    }
+    return r;
+  }
+};
+template <>
+struct Eight<Elem::f32> {
+  float x[8];
+  __device__ __forceinline__ void load4(const void* p, int half) { load_elems<Elem::f32, 4>(static_cast<const float*>(p), x + 4 * half); }
+  __device__ __forceinline__ void set(int e, float v) { x[e] = v; }
+  __device__ __forceinline__ void clear_from(int n) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e >= n ? 0.f : x[e];
+  }
+  __device__ __forceinline__ uint32_t abs_max() const { return abs_max8(x); }
+  __device__ __forceinline__ void floats(float* y) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e];
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const { return codes8(x, scale); }
+};
+
 template <Elem E, int M>
 __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Cache c, Kv4Rows k, Kv4Rows v, int64_t rows, const int64_t* slots, int vec) {
   typedef typename ElemOf<E>::T T;
@@ -162,40 +226,43 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4Cache c, Kv4Rows k, K
   const bool in = it.r < rows && it.h < c.heads;
   const T* kp = static_cast<const T*>(k.p) + it.r * k.row + it.h * k.head;
   const T* vp = static_cast<const T*>(v.p) + it.r * v.row + it.h * v.head;
-  float x[2][8];
+  Eight<E> x[2];
+  x[0].clear_from(0), x[1].clear_from(0);
   // (loads are clamped into the row and selected afterwards: none waits for another)
   if (in && vec) {
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
       const int d = d0 + e + 4 <= c.head_dim ? d0 + e : c.head_dim - 4;
-      load_elems<E, 4>(kp + d, &x[0][e]);
-      load_elems<E, 4>(vp + d, &x[1][e]);
+      x[0].load4(kp + d, e >> 2);
+      x[1].load4(vp + d, e >> 2);
     }
   } else if (in) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = d0 + e < c.head_dim ? d0 + e : c.head_dim - 1;
-      x[0][e] = ElemOf<E>::get(kp[d * k.elem]);
-      x[1][e] = ElemOf<E>::get(vp[d * v.elem]);
+      x[0].set(e, kp[d * k.elem]);
+      x[1].set(e, vp[d * v.elem]);
     }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (!in || d0 + e >= c.head_dim) x[0][e] = x[1][e] = 0.f;
+  x[0].clear_from(c.head_dim - d0), x[1].clear_from(c.head_dim - d0);
   item_run(it);
   uint32_t codes[2], scale[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    uint32_t a = abs_max8(x[w]);
-    if (a >= 0x7f800000u) {   // an infinity or NaN: rare
+    const uint32_t own = x[w].abs_max();
+    uint32_t a = own;
+    float y[8];
+    if (own >= 0x7f800000u) {   // an infinity or NaN: rare
+      x[w].floats(y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[w][e] = storable(x[w][e]);
-      a = abs_max8(x[w]);
+      for (int e = 0; e < 8; ++e) y[e] = storable(y[e]);
+      a = abs_max8(y);
     }
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0xB1 /* quad_perm 1,0,3,2 */, 0xf, 0xf, false));
     a = max(a, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, 0x4E /* quad_perm 2,3,0,1 */, 0xf, 0xf, false));
     scale[w] = scale_byte(a);
-    codes[w] = codes8(x[w], kv4_scale(scale[w]));
+    codes[w] = x[w].codes(kv4_scale(scale[w]));
+    if (own >= 0x7f800000u) codes[w] = codes8(y, kv4_scale(scale[w]));
   }
   const uint32_t run = transpose4(codes[1], it.tok);   // (every lane takes part in the exchange)
   if (!it.live) return;
