@@ -514,7 +514,7 @@ __global__ __launch_bounds__(256, (waves_wanted<M, E, RT>())) void kv4_attention
 // The same walk for many rows: a workgroup has 64 * RT rows, a wave 16 * RT of them, and all four walk the same blocks.  The matrix operands of
 // a block are expanded ONCE, a quarter by each wave, into shared memory (in the order in which a wave reads them back: 16 bytes a lane, no
 // conflicts), two blocks deep: one barrier a block, the bytes of later blocks in flight meanwhile.
-// 4 sequences of 2500 to 8191 tokens with 485 to 1000 queries, 32 over 8 heads of 128, f16: 560 us and 39 for the join, 480 TFLOP/s of the formula's
+// 4 sequences of 2500 to 8191 tokens with 485 to 1000 queries, 32 over 8 heads of 128, f16: 550 us and 36 for the join, 490 TFLOP/s of the formula's
 // products.  Two terms of q and of p make each of them two on the matrix unit, which is busy half of the time and the vector unit (softmax, terms, expanding)
 // the other half, at 2.1 GHz: what is left is their overlap.  Each wave expanding for itself: 740 us; operands read where they are used: 720.
 // a wave's quarter of a block: keys' operands wave, wave + 4, ... of 2 M and values' groups (wave + 2) % 4, + 4, ... of M
@@ -727,14 +727,15 @@ __global__ __attribute__((amdgpu_waves_per_eu((M <= 4 ? 2 : 1), (M <= 4 ? 2 : 1)
   put_walk<M, E, RT>(a, split, w, row0, n_rows, q0, head, per, lane);
 }
 
-// Joins the key ranges of one (row, head): one wave each.  What it waits for is loads, so all are on their way before the first is used, the row's
-// owner looked up meanwhile.
+// Joins the key ranges of one (row, head): one wave each, or the WAVES = 4 of a workgroup where rows are few and ranges many.  What it waits for is loads, so
+// all are on their way before the first is used, the row's owner looked up meanwhile.  96 rows of 256, 26 ranges: 5.4 us by four waves, 10.4 by one; 512 rows of
+// 128, 15 ranges: 4.8 and 5.1; 95040 rows of 128, two ranges, one wave each: 36 us, 3.4 TB/s.
 // kFirst: turns whose loads do not wait for anything (one where one is all there is)
-template <Elem E, int kFirst>
+template <Elem E, int kFirst, int WAVES>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   typedef typename ElemOf<E>::T T;
-  const int lane = threadIdx.x & 63;
-  const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = WAVES > 1 ? wave : 0;
+  const uint32_t id = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
   const uint32_t row = id / (uint32_t)a.heads;
   const int h = (int)(id - row * a.heads);
   if (row >= a.rows) return;
@@ -746,7 +747,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   // the shuffles read lanes of all groups.)
   const int per = dp >> 2, groups = 64 / per, group = lane / per, d0 = (lane - group * per) * 4;
   const bool has = group < groups;
-  auto piece = [&](int turn) { return *reinterpret_cast<const float4*>(p + min(turn * groups + (has ? group : 0), a.nsplit - 1) * stride + d0); };
+  auto range = [&](int turn) { return (turn * groups + (has ? group : 0)) * WAVES + part; };
+  auto piece = [&](int turn) { return *reinterpret_cast<const float4*>(p + min(range(turn), a.nsplit - 1) * stride + d0); };
   float4 first[kFirst];
 #pragma unroll
   for (int i = 0; i < kFirst; ++i) first[i] = piece(i);
@@ -774,11 +776,11 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   float4 v{0.f, 0.f, 0.f, 0.f};
   auto add = [&](int turn, const float4& x) {
-    const int s = turn * groups + (has ? group : 0);
+    const int s = range(turn);
     const float g = __shfl(f, s & 63);
     if (s < a.nsplit && has) v.x += x.x * g, v.y += x.y * g, v.z += x.z * g, v.w += x.w * g;
   };
-  const int turns = (a.nsplit + groups - 1) / groups;
+  const int turns = (a.nsplit + groups * WAVES - 1) / (groups * WAVES);
 #pragma unroll
   for (int i = 0; i < kFirst; ++i) add(i, first[i]);
   if (kFirst > 1) {
@@ -788,6 +790,17 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4Attention a, int dp) {
   for (int k = 1; k < groups; ++k) {
     const float4 x{__shfl(v.x, lane + k * per), __shfl(v.y, lane + k * per), __shfl(v.z, lane + k * per), __shfl(v.w, lane + k * per)};
     if (group == 0) v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+  }
+  if constexpr (WAVES > 1) {
+    __shared__ float4 sums[WAVES][64];
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const float4 x = sums[w][lane];
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    }
   }
   if (group == 0) {
     T* o = static_cast<T*>(a.out) + (int64_t)row * a.out_row + h * a.out_head;
@@ -832,9 +845,13 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
     else if (shape.rt == 1) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 1>), grid, dim3(256), 0, s, a);
     else if constexpr (M <= 2 || E != Elem::f32) MSH_LAUNCH((kv4_attention_kernel<M, E, 2, 4>), grid, dim3(256), 0, s, a);   // (kv4_attention_shape())
   }
-  const dim3 rows4((unsigned)((a.rows * a.heads + 3) / 4));
-  if (a.nsplit > 1 && a.nsplit <= 64 / (8 * M)) MSH_LAUNCH((kv4_join_kernel<E, 1>), rows4, dim3(256), 0, s, a, 32 * M);
-  else if (a.nsplit > 1) MSH_LAUNCH((kv4_join_kernel<E, 4>), rows4, dim3(256), 0, s, a, 32 * M);
+  if (a.nsplit == 1) return;
+  const int64_t joins = a.rows * a.heads;
+  const dim3 by_wave((unsigned)((joins + 3) / 4)), by_group((unsigned)joins);
+  constexpr int groups = 64 / (8 * M);   // ranges that a wave takes at a time
+  if (a.nsplit > 2 * groups && joins <= 1024) MSH_LAUNCH((kv4_join_kernel<E, 4, 4>), by_group, dim3(256), 0, s, a, 32 * M);
+  else if (a.nsplit > groups) MSH_LAUNCH((kv4_join_kernel<E, 4, 1>), by_wave, dim3(256), 0, s, a, 32 * M);
+  else MSH_LAUNCH((kv4_join_kernel<E, 1, 1>), by_wave, dim3(256), 0, s, a, 32 * M);
 }
 
 template <Elem E>
