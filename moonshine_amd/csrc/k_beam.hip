@@ -1,6 +1,7 @@
 // Beam search: selection over beams and vocabulary, reordering of the states that the selected beams continue.
 #include <float.h>
 
+#include "beam_list.h"
 #include "kernels.h"
 #include "kv4_common.h"
 
@@ -36,8 +37,6 @@ struct Entry {
 };
 __host__ __device__ inline size_t part_bytes(int beams) { return sizeof(Part) + sizeof(Entry) * ((beams + 1) & ~1); }   // (16-byte multiples)
 
-constexpr int kLane = 32;                                      // elements of a lane per chunk
-constexpr int kListMax = 2 * kBeamMax + kBeamMax * (kLane + 1);   // room for one chunk's most beside 2 K
 constexpr int kPartsMax = 64;                                  // a row's parts lie in one wave of pass 2
 
 __device__ __forceinline__ bool before(const Entry& a, const Entry& b) { return a.val > b.val || (a.val == b.val && a.idx < b.idx); }
@@ -180,16 +179,17 @@ __global__ __launch_bounds__(256, (E == Elem::f32 ? 4 : 5)) void beam_partial_ke
     }
     sum += (double)part_sum;
 
-    // what is above the bound joins the list; until K elements are known to reach it, the K-th largest lane maximum becomes the bound
-    const int over = __popcll(__builtin_amdgcn_ballot_w64(hi > bound));
+    // what is above the bound joins the list; where the list's room asks for it (beam_list.h), the K-th largest lane maximum becomes the bound
+    int over = __popcll(__builtin_amdgcn_ballot_w64(hi > bound));
     if (over == 0) continue;
-    if (n > kListMax - K * (kLane + 1)) {   // (a chunk adds K * 32 elements and K ties at most)
+    if (beam_list_cut(n, K)) {
       n = rank_list(list, best, n, K, lane);
       if (lane < n) list[lane] = best[lane];
       if (n == K) bound = fmaxf(bound, best[K - 1].val), enough = true;
       wave_fence();
+      over = __popcll(__builtin_amdgcn_ballot_w64(hi > bound));
     }
-    const bool raise = over > K && !enough;
+    const bool raise = beam_bound_rises(n, K, over, enough);   // (more than K lanes are above the bound: it rises)
     if (raise) bound = wave_kth(hi, K, lane);
     const int n0 = n;
 #pragma unroll

@@ -4,6 +4,7 @@
 // allocated, copied or waited for, so all of them may be captured into a graph.
 #pragma once
 
+#include "beam_list.h"
 #include "msh_common.h"
 
 namespace msh {
@@ -92,7 +93,6 @@ struct BeamSelect {
   int32_t batch, beams, vocab, eos;
   bool fixed = false;         // as in Kv4Attention
 };
-constexpr int kBeamMax = 16;
 size_t beam_select_work_bytes(int batch, int beams, int vocab, bool fixed = false);
 void beam_select(const BeamSelect& a, Elem type, hipStream_t s);
 
