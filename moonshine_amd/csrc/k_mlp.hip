@@ -26,6 +26,7 @@
 #include <vector>
 
 #include "gemm_common.h"
+#include "mlp_schedule.h"
 #include "panel_rows.h"
 
 namespace msh {
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(256, 1) void mlp_fused_kernel(float* __restrict__ H
   //   * the fragments, read from LDS in consumption order through a ring of PF register sets (PF reads ahead, counted
   //     lgkmcnt, piece offset in the instruction's immediate) -- ACROSS stage boundaries: the ring never drains;
   //   * GELU of chunk j (vector pipe), spread over the fc2 MFMAs of chunk j-1 (matrix pipe), which do not depend on it;
-  //   * ONE workgroup barrier, in the MIDDLE of the stage: it publishes stage j+1 (every wave has waited for its own
+  //   * ONE workgroup barrier, in the MIDDLE of the stage (mlp_schedule.h): it publishes stage j+1 (every wave has waited for its own
   //     pieces, issued half a stage earlier) and retires stage j-1, whose buffer the DMAs of stage j+2 then refill, one
   //     every other MFMA of the second half.  At the stage boundary itself there is no synchronisation at all (a barrier
   //     there cost ~450 cycles per stage: the matrix pipe ran dry while the first fragments of the new stage were read).
@@ -239,7 +240,8 @@ __global__ __launch_bounds__(256, 1) void mlp_fused_kernel(float* __restrict__ H
   auto stage = [&](int j, int buf, auto kind_c, int next_f0) {
     constexpr int KIND = decltype(kind_c)::value;
     constexpr bool DO1 = KIND != 2, DO2 = KIND != 0, LAST = KIND == 2;
-    constexpr int F0 = DO1 ? 0 : KS, NF = (DO1 ? KS : 0) + (DO2 ? KS : 0), MID = NF / 2;
+    constexpr int F0 = DO1 ? 0 : KS, NF = (DO1 ? KS : 0) + (DO2 ? KS : 0), MID = mlp_publish_step(NF, PF, LAST);
+    static_assert(MID >= 0 && (LAST || NF - PF >= MID), "the next stage's fragments are read before they are published");
     // slot of step f in the fragment ring: the ring runs on across stages, the first stage is KS steps long, every other
     // one 2 KS (a multiple of PF), the last one KS again
     constexpr int RO = KIND == 0 ? 0 : KS % PF;
@@ -344,7 +346,8 @@ __global__ __launch_bounds__(256, 1) void mlp_fused_kernel(float* __restrict__ H
       }
       static_for<NOP>([&](auto ic) {
         constexpr int I = decltype(ic)::value, T0 = 2 * I, T1 = 2 * I + 1 < CT ? 2 * I + 1 : CT - 1;   // (a missing last tile: zero weights)
-        constexpr int NF = 2 * KS, MID = NF / 2;
+        constexpr int NF = 2 * KS, MID = mlp_publish_step(NF, PF, false);
+        static_assert(MID >= 0 && NF - PF >= MID, "the next stage's fragments are read before they are published");
         static_assert(NF % PF == 0, "an o-proj stage must leave the fragment ring's phase unchanged");
         constexpr int DS = (ABL & 16) ? 0 : ((NF - MID - 2) / NG > 0 ? (NF - MID - 2) / NG : 1);
         const int nbuf = buf + 1 == NST ? 0 : buf + 1;
