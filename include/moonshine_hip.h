@@ -363,7 +363,7 @@ MSH_EXPORT int32_t msh_page_plan(int32_t device, void* stream, int32_t* block_ta
 
 /* Write `rows` keys and values [rows][heads][head_dim] (element strides: row, head, element) into their slots; a slot that is negative
  * or past the cache is skipped.  The slots of a call must differ (else the token is one of the rows' or a mix of them).  NaN is
- * stored as 0, infinities as the largest finite value; a group below 2^-102 becomes 0.
+ * stored as 0, infinities as the largest finite value; a group below 2^-102 becomes 0.  At most 2^26 - 32 rows a call.
  * msh_kv4_read: the values of slots, contiguous [rows][heads][head_dim]; zeros for a slot that is not in the cache. */
 MSH_EXPORT int32_t msh_kv4_write(int32_t device, void* stream, const msh_kv4_cache* cache, const void* k, const int64_t* k_strides,
                                  const void* v, const int64_t* v_strides, int32_t dtype, int64_t rows, const int64_t* slots);

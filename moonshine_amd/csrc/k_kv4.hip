@@ -362,7 +362,7 @@ void kv4_write(const Kv4Cache& c, const Kv4Rows& k, const Kv4Rows& v, Elem type,
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
   const int vec = k.elem == 1 && v.elem == 1 && by_fours(k.p, {k.row, k.head}, c.head_dim, size) && by_fours(v.p, {v.row, v.head}, c.head_dim, size);
-  const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
+  const dim3 grid((unsigned)kv4_rows_groups(rows), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
   by_groups(kv4_groups(c.head_dim), [&](auto m) {
     constexpr int M = decltype(m)::value;
     if (type == Elem::f32) MSH_LAUNCH((kv4_write_kernel<Elem::f32, M>), grid, dim3(256), 0, s, c, k, v, rows, slots, vec);
@@ -375,7 +375,7 @@ void kv4_read(const Kv4Cache& c, const int64_t* slots, int64_t rows, void* k, vo
   if (rows == 0) return;
   const size_t size = elem_bytes(type);
   const int vec = by_fours(k, {}, c.head_dim, size) && by_fours(v, {}, c.head_dim, size);
-  const dim3 grid((unsigned)((rows + 31) / 32 * 8), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
+  const dim3 grid((unsigned)kv4_rows_groups(rows), (unsigned)((c.heads * kv4_groups(c.head_dim) + 15) / 16));
   by_groups(kv4_groups(c.head_dim), [&](auto m) {
     constexpr int M = decltype(m)::value;
     if (type == Elem::f32) MSH_LAUNCH((kv4_read_kernel<Elem::f32, M>), grid, dim3(256), 0, s, c, slots, rows, k, v, vec);
@@ -421,7 +421,7 @@ Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
 // 485 to 1000 queries: 529 against 617; all of 8192: 771 against 752; at 2048 tokens the join would cost a quarter: 260 against 207).
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   const Kv4Shape shape = kv4_attention_shape(a, type);
-  if (a.fixed || shape.kw != 4 || a.rows * a.heads >= (1 << 26)) return 1;   // (a grid has 2^32 threads)
+  if (a.fixed || shape.kw != 4 || kv4_join_groups(a.rows, a.heads) > kGroupsMost) return 1;
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
   const int64_t units = (int64_t)a.batch * a.cache.heads * ((rows + shape.rows() - 1) / shape.rows());
   const int64_t room = (int64_t)a.width << a.cache.page_shift;
@@ -433,6 +433,12 @@ int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   int64_t n = wanted / units;
   n = n < room / least ? n : room / least;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+}
+int64_t kv4_attention_groups(const Kv4Attention& a, Elem type) {
+  const Kv4Shape shape = kv4_attention_shape(a, type);
+  const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads), pairs = (int64_t)a.batch * a.cache.heads;
+  const int64_t units = pairs * ((rows + shape.rows() - 1) / shape.rows()), per_group = 4 / shape.kw;
+  return shape.chunk ? (pairs + 7) / 8 * 8 * (units / pairs) * a.nsplit : (units + per_group - 1) / per_group;   // (chunks: the second axis is in the first)
 }
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit) {
   return nsplit > 1 ? (size_t)a.rows * a.heads * nsplit * (32 * kv4_groups(a.cache.head_dim) + kPartPad) : 0;

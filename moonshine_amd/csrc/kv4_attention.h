@@ -825,7 +825,6 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
   Kv4Attention a = a0;
   const Kv4Shape shape = kv4_attention_shape(a, E);
   const int64_t rows = (int64_t)a.max_q * (a.heads / a.cache.heads);
-  const int64_t pairs = (int64_t)a.batch * a.cache.heads;
   a.tiles = (int32_t)((rows + shape.rows() - 1) / shape.rows());
   const int64_t four = E == Elem::f32 ? 16 : 8;   // bytes of four elements
   const int64_t size = four / 4;
@@ -835,11 +834,10 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
   a.sign = a.scale_log2 < 0.f ? -1.f : 1.f;
   a.scale_log2 = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);   // (0 * -inf of a masked score would be NaN; any score times this is 0 to exp2)
   if (shape.chunk) {
-    const dim3 grid((unsigned)((pairs + 7) / 8 * 8 * a.tiles * a.nsplit));
+    const dim3 grid((unsigned)kv4_attention_groups(a, E));
     MSH_LAUNCH((kv4_attention_chunk_kernel<M, E, 2>), grid, dim3(256), 0, s, a);
   } else {
-    const int64_t per_group = 4 / shape.kw;
-    const dim3 grid((unsigned)((pairs * a.tiles + per_group - 1) / per_group), (unsigned)a.nsplit);
+    const dim3 grid((unsigned)kv4_attention_groups(a, E), (unsigned)a.nsplit);
     if (shape.rt == 1 && shape.kw == 4) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 4>), grid, dim3(256), 0, s, a);
     else if (shape.rt == 1 && shape.kw == 2) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 2>), grid, dim3(256), 0, s, a);
     else if (shape.rt == 1) MSH_LAUNCH((kv4_attention_kernel<M, E, 1, 1>), grid, dim3(256), 0, s, a);
@@ -847,7 +845,7 @@ void launch_kv4_attention(const Kv4Attention& a0, hipStream_t s) {
   }
   if (a.nsplit == 1) return;
   const int64_t joins = a.rows * a.heads;
-  const dim3 by_wave((unsigned)((joins + 3) / 4)), by_group((unsigned)joins);
+  const dim3 by_wave((unsigned)kv4_join_groups(a.rows, a.heads)), by_group((unsigned)joins);
   constexpr int groups = 64 / (8 * M);   // ranges that a wave takes at a time
   if (a.nsplit > 2 * groups && joins <= 1024) MSH_LAUNCH((kv4_join_kernel<E, 4, 4>), by_group, dim3(256), 0, s, a, 32 * M);
   else if (a.nsplit > groups) MSH_LAUNCH((kv4_join_kernel<E, 4, 1>), by_wave, dim3(256), 0, s, a, 32 * M);

@@ -96,7 +96,11 @@ msh::Kv4Attention attention_of(const msh_kv4_attention_args* x, msh::Elem* type)
   a.rows = x->rows, a.heads = x->heads, a.batch = x->batch, a.width = x->table_width, a.max_q = x->max_q;
   a.causal = x->causal != 0, a.window = x->window;
   a.scale_log2 = x->scale * 1.44269504088896341f;
-  a.nsplit = x->rows == 0 || x->batch == 0 ? 1 : msh::kv4_attention_splits(a, *type);
+  a.nsplit = 1;
+  if (x->rows > 0 && x->batch > 0) {
+    a.nsplit = msh::kv4_attention_splits(a, *type);
+    need(msh::kv4_attention_groups(a, *type) <= msh::kGroupsMost, "the call is too large for one launch");
+  }
   return a;
 }
 
@@ -137,7 +141,7 @@ int32_t msh_kv4_write(int32_t device, void* stream, const msh_kv4_cache* cache, 
   return op_guarded([&] {
     const msh::Kv4Cache c = cache_of(cache);
     const msh::Elem t = elem(dtype);
-    need(rows >= 0 && rows < (1 << 26), "rows: 0 to 2^26 - 1");
+    need(rows >= 0 && rows <= kMost && msh::kv4_rows_groups(rows) <= msh::kGroupsMost, "rows: 0 to 2^26 - 32");
     if (rows == 0) return;
     need(k && v && k_strides && v_strides && slots, "null pointer");
     DeviceScope scope(device);
@@ -151,7 +155,7 @@ int32_t msh_kv4_read(int32_t device, void* stream, const msh_kv4_cache* cache, c
   return op_guarded([&] {
     const msh::Kv4Cache c = cache_of(cache);
     const msh::Elem t = elem(dtype);
-    need(rows >= 0 && rows < (1 << 26), "rows: 0 to 2^26 - 1");
+    need(rows >= 0 && rows <= kMost && msh::kv4_rows_groups(rows) <= msh::kGroupsMost, "rows: 0 to 2^26 - 32");
     if (rows == 0) return;
     need(k && v && slots, "null pointer");
     DeviceScope scope(device);

@@ -79,6 +79,11 @@ Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type);
 // number of key ranges a launch is split into, and the floats of workspace that takes
 int kv4_attention_splits(const Kv4Attention& a, Elem type);
 size_t kv4_attention_part_floats(const Kv4Attention& a, int nsplit);
+// workgroups of 256 threads along the first axis of a launch: a grid has fewer than 2^32 threads there
+constexpr int64_t kGroupsMost = ((int64_t)1 << 24) - 1;
+inline int64_t kv4_rows_groups(int64_t rows) { return (rows + 31) / 32 * 8; }                       // of a write or read
+inline int64_t kv4_join_groups(int64_t rows, int heads) { return (rows * heads + 3) / 4; }          // of the join, a wave per (row, head)
+int64_t kv4_attention_groups(const Kv4Attention& a, Elem type);                                     // of the attention, `nsplit` set
 void kv4_attention(const Kv4Attention& a, Elem type, hipStream_t s);
 
 struct BeamSelect {
