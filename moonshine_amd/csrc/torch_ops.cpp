@@ -83,6 +83,11 @@ void no_grad(const at::Tensor& t) {
     refuse("an input requires a gradient: this operator has no backward pass (call it under torch.no_grad())");
 }
 
+// a tensor that the call writes in place counts as changed, so that a backward pass that saved it says so.  (One made under inference mode has no count.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int32_t dtype_of(const at::Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kFloat: return MSH_F32;
@@ -155,6 +160,7 @@ PyObject* page_plan(PyObject* const* a) {
   at::Tensor slots = make(p, {rows}, at::kLong), used = make(p, {1}, at::kInt);
   check(msh_page_plan(p.device, p.stream, tp, small(batch, "batch"), small(width, "width"), kp, fp, sp, rows, pp, n_free, small(page, "page_size"),
                       (int64_t*)slots.data_ptr(), (int32_t*)used.data_ptr()));
+  written(table);
   return wrap({slots, used});
 }
 
@@ -172,6 +178,7 @@ PyObject* kv4_write(PyObject* const* a) {
   auto* sp = (const int64_t*)array(slots, "slots", at::kLong, {rows});
   const int64_t ks[3] = {k.stride(0), k.stride(1), k.stride(2)}, vs[3] = {v.stride(0), v.stride(1), v.stride(2)};
   check(msh_kv4_write(p.device, p.stream, &c, k.data_ptr(), ks, v.data_ptr(), vs, type, rows, sp));
+  written(cache);
   Py_RETURN_NONE;
 }
 
@@ -249,6 +256,7 @@ PyObject* kv4_attention(PyObject* const* a) {
   const int64_t size = check(msh_kv4_attention_workspace(&x));
   const c10::DataPtr work = size > 0 ? allocator()->allocate((size_t)size) : c10::DataPtr();
   check(msh_kv4_attention(p.device, p.stream, &x, work.get(), size));
+  if (a[10] != Py_None) written(out);
   if (with_lse) return wrap({out, lse});
   return THPVariable_Wrap(out);
 }
@@ -330,6 +338,7 @@ PyObject* beam_reorder(PyObject* const* a) {
     each = lengths.size(0) == batch ? 1 : 0;
   }
   check(msh_beam_reorder(p.device, p.stream, states, (int32_t)n, small(batch, "batch"), small(beams, "beams"), pp, lp, each));
+  for (Py_ssize_t i = 0; i < n; ++i) written(tensor(PyList_GET_ITEM(a[0], i), "state"));
   Py_RETURN_NONE;
 }
 
