@@ -7,6 +7,7 @@
 #include <ATen/EmptyTensor.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -81,6 +82,9 @@ struct Place {
 void no_grad(const at::Tensor& t) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse("an input requires a gradient: this operator has no backward pass (call it under torch.no_grad())");
+  // (torch.no_grad() does not end forward differentiation)
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+    refuse("an input has a tangent: this operator has no forward derivative");
 }
 
 // a tensor that the call writes in place counts as changed, so that a backward pass that saved it says so.  (One made under inference mode has no count.)

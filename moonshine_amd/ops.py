@@ -3,9 +3,8 @@ selection and state reordering of a beam search (include/moonshine_hip.h, "servi
 
 Every call runs on the tensors' device and on torch's current stream there, enqueues and returns: no synchronisation, no state
 between calls, results independent of what else runs; all of it may be captured into a graph.  Outputs and workspaces come from
-torch's allocator.  There is no backward pass: inputs that require a gradient are refused; what a call writes in place counts as changed
-to autograd.  A refused argument raises
-``MshError`` (code -3) before anything is launched.
+torch's allocator.  There is no backward pass: inputs that require a gradient, or have a tangent of forward differentiation, are refused;
+what a call writes in place counts as changed to autograd.  A refused argument raises ``MshError`` (code -3) before anything is launched.
 
 A decode step over a paged cache::
 

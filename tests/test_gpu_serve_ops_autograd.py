@@ -1,9 +1,11 @@
 """The serving operators beside torch's own bookkeeping: what they write in place counts as changed (a backward pass that saved it says so instead of
-using the new values)."""
+using the new values), and inputs whose derivative they would drop are refused."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from moonshine_amd import ops
+from moonshine_amd.hip_api import MshError
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +64,27 @@ def test_tensors_made_under_inference_mode():
     ops.beam_reorder(s.states, s.parents, batch_dims=[0, 0], row_dims=[2, 2])     # they have no version to count
     ops.kv4_write(s.cache, s.k, s.v, s.slots)
     assert s.states[0].is_inference()
+
+
+def inputs():
+    """name -> (a call that takes the tensor, the tensor)"""
+    s = Setting()
+    return {"k": (lambda x: ops.kv4_write(s.cache, x, s.v, s.slots), s.k), "v": (lambda x: ops.kv4_write(s.cache, s.k, x, s.slots), s.v),
+            "q": (lambda x: ops.kv4_attention(x, s.cache, s.table, s.lens), s.q),
+            "out": (lambda x: ops.kv4_attention(s.q, s.cache, s.table, s.lens, out=x), torch.zeros_like(s.q)),
+            "logits": (lambda x: ops.beam_select(x, s.scores, s.finished, 2), s.logits), "scores": (lambda x: ops.beam_select(s.logits, x, s.finished, 2), s.scores),
+            "state": (lambda x: ops.beam_reorder([x], s.parents, batch_dims=[0], row_dims=[2]), s.states[0])}
+
+
+NAMES = ["k", "v", "q", "out", "logits", "scores", "state"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_forward_derivative_is_not_dropped(name):
+    call, x = inputs()[name]
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(MshError, match="forward") as e:
+            call(dual)
+        assert e.value.code == -3
+    call(x)
