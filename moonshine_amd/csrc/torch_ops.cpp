@@ -43,7 +43,9 @@ std::string shape_of(const at::Tensor& t) {
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(std::string(name) + ": a tensor is wanted");
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.is_neg() || t.is_conj()) refuse(std::string(name) + ": a view whose sign torch has not applied yet (x.conj().imag); give x.resolve_neg()");
+  return t;
 }
 int64_t integer(PyObject* o, const char* name) {
   const int64_t v = PyLong_AsLongLong(o);

@@ -1,5 +1,5 @@
 """The serving operators beside torch's own bookkeeping: what they write in place counts as changed (a backward pass that saved it says so instead of
-using the new values), and inputs whose derivative they would drop are refused."""
+using the new values), and inputs whose derivative or pending sign they would drop are refused."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -88,3 +88,15 @@ def test_a_forward_derivative_is_not_dropped(name):
             call(dual)
         assert e.value.code == -3
     call(x)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_pending_sign_is_not_dropped(name):
+    """The imaginary part of a conjugate is a view whose sign torch has not applied yet: its memory holds the other sign."""
+    call, x = inputs()[name]
+    z = torch.complex(torch.zeros_like(x), -x).conj().imag
+    assert z.is_neg() and torch.equal(z, x)
+    with pytest.raises(MshError, match="sign") as e:
+        call(z)
+    assert e.value.code == -3
+    call(z.resolve_neg().contiguous())
