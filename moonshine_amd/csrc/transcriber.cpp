@@ -604,6 +604,7 @@ Transcriber::Transcriber(const TranscriberOptions& options) : opt_(options) {
 // json and tokenizer, core/moonshine-streaming-model.cpp:233-300).
 void Transcriber::load_streaming_model() {
   if (opt_.beam_width != 1) throw std::runtime_error("beam_width: the streaming architectures decode greedily (their drafts are verified against it)");
+  if (opt_.kv_dtype == 2) throw std::runtime_error("kv_dtype: the streaming architectures have no mxfp4 cache (their cross K / V are bf16)");
   // (word_timestamps: the reference swaps in decoder_kv_with_attention.ort here, core/transcriber.cpp:327-345; this engine
   //  computes the attention of the final token sequence on request, StreamingEngine::cross_attention)
   const int frames = (int)ceilf(opt_.max_stream_seconds * 50.0f);
