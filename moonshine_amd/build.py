@@ -130,24 +130,36 @@ def check_no_packed_fp32(objs: list[str]) -> dict[str, int]:
     return seen
 
 
-def build_ops(force: bool = False) -> str:
-    """msh_torch_ops.so: the module behind moonshine_amd.ops.  Host code only; finds libmoonshine.so beside itself."""
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "moonshine_hip.h")))
-    if not force and os.path.exists(LIB_OPS) and os.path.getmtime(LIB_OPS) > newest:
-        return LIB_OPS
+def build_ops(force: bool = False) -> str | None:
+    """msh_torch_ops.so: the module behind moonshine_amd.ops, for the torch that is installed.  Host code only; finds libmoonshine.so beside
+    itself.  Without torch or its headers there is no such module (None), and the library, which needs neither, builds all the same."""
     import sysconfig
 
-    import torch
-
+    try:
+        import torch
+    except ImportError as e:
+        print(f"moonshine_amd.ops is not built: no torch ({e})", file=sys.stderr)
+        return None
     root = os.path.dirname(torch.__file__)
+    if not os.path.exists(os.path.join(root, "include", "ATen", "ATen.h")):
+        print(f"moonshine_amd.ops is not built: no torch headers under {root}", file=sys.stderr)
+        return None
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "moonshine_hip.h")))
+    built_for = f"torch {torch.__version__} at {root}, python {sys.version_info.major}.{sys.version_info.minor}\n"
+    stamp = LIB_OPS + ".torch"
+    same = os.path.exists(stamp) and open(stamp).read() == built_for
+    if not force and same and os.path.exists(LIB_OPS) and os.path.getmtime(LIB_OPS) > newest:
+        return LIB_OPS
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{root}/include",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DMSH_TORCH_VERSION="{torch.__version__}"', f"-I{INCLUDE}", f"-I{root}/include",
            f"-I{root}/include/torch/csrc/api/include", "-I/opt/rocm/include", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{sysconfig.get_paths()['include']}", src, "-o", LIB_OPS,
            f"-L{LIBDIR}", "-l:libmoonshine.so", f"-L{root}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10_hip", "-lc10", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return LIB_OPS
 
 

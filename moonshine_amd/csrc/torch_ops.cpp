@@ -395,4 +395,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "msh_torch_ops", nullptr, -1, metho
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit_msh_torch_ops() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit_msh_torch_ops() {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", MSH_TORCH_VERSION) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

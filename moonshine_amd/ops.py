@@ -39,6 +39,8 @@ def _load():
     spec = importlib.util.spec_from_file_location("msh_torch_ops", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.torch_version != torch.__version__:
+        raise ImportError(f"{path} was built for torch {module.torch_version}, this is {torch.__version__}: run `python -m moonshine_amd.build`")
     module.set_up(MshError)
     return module
 
