@@ -17,6 +17,8 @@ constexpr bool beam_list_cut(int n, int K) { return n > kListMax - K * (kLane + 
 //   bound raised:      fewer than K lanes stay above it, (K - 1) kLane elements, and ties fill up to K:  at most K (kLane + 1)
 //   over <= K lanes:   K kLane elements
 //   otherwise:         n + over kLane <= kListMax, checked here
+// Measured, us a call: raised for every chunk with more than K lanes above it, 256 x 8 beams over 32768 bf16 logits 56 instead of 53, 1 x 7 over 193263 19.5
+// instead of 18.3; asked for less often, by a list of 900 entries, 1 x 16 over 193001 68 instead of 42 (longer lists to rank).
 constexpr bool beam_bound_rises(int n, int K, int over, bool enough) { return over > K && (!enough || n + over * kLane > kListMax); }
 
 }  // namespace msh

@@ -18,12 +18,14 @@ __device__ __forceinline__ void wave_fence() {   // shared memory written by one
 // Pass 1, one wave per (row, part): running maximum and sum of exponentials, and the part's `beams` best logits in order -- the order
 //   inside a row does not depend on its sum.  Elements stay in registers (32 a lane); the next 32 are in flight.  The K-th largest of
 //   the 64 lanes' maxima bounds the K-th largest element from below, so that all but a handful are dismissed by one comparison;
-//   later elements are held against that bound, and the list of what passed is ranked once.  One read of the logits: bound by HBM bandwidth for batches, by
-//   latency (and the fetch of its own instructions: rare paths are loops, not copies) for one clip.
+//   later elements are held against that bound, which rises again where what passes could fill the list (beam_list.h), and the list of what passed is
+//   ranked once.  One read of the logits.  Bound by the vector unit for batches (61 % busy: 19 instructions for 64 logits, fixed work of each part among
+//   them), by latency (and the fetch of its own instructions: rare paths are loops, not copies) for one clip.
 // Pass 2, one workgroup per batch entry, a thread per (row, part): joins the rows' sums, takes from the parts' lists what reaches the K-th
 //   largest list head of a wave, ranks those few by counting.  Bound by the latency of its chain of steps.
-// 256 entries of 8 beams over 32768 bf16 logits (a sixth of the beams finished: 114 MB): 40 us, 2.8 TB/s, and 9.6 us; 1 entry of 4 beams, 32-bit logits:
-// 6.9 and 3.9 us; 1 entry of 7 beams over 193001: 11 and 6 us.
+// 256 entries of 8 beams over 32768 bf16 logits (a sixth of the beams finished: 114 MB): 41 us, 2.8 TB/s, and 9.6 us; 1 entry of 4 beams, 32-bit logits:
+// 6.6 and 4.0 us; 1 entry of 7 beams over 193263 (bf16): 10.4 and 6.2 us; 17 of 10 over 86111: 19.3 and 8.2 us.  Logits that rise all along a row, so that
+// every chunk passes the bound of the one before, are the dearest: the first of these takes 133 us a call instead of 53.
 // The sums are added in 64 bits from 32 exponentials at a time and the scores compared in 64 bits: the order of two candidates of
 // different beams hangs on both rows' sums.
 struct Part {

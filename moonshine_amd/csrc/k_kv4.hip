@@ -9,7 +9,8 @@ namespace {
 // kept_b + i of request b becomes free[first_b + i], and the row at place p of request b the slot table[b][p / P] * P + p mod P.
 // One launch, one workgroup per request: each adds up the lengths of the requests before it for itself (8 bytes each, out of L2) instead of
 // waiting for a scan of its own launch, and clears the rows between its own and the next request's.  A few bytes per request: bound by
-// launch and memory latency.  5 requests 2.9 us, 1999 with up to 16000 tokens each 6.2 us.
+// launch and memory latency.  5 requests 2.9 us, 1999 with up to 16000 tokens each 6.1 us.  (The sums grow with the square of the requests: a plan of tens of
+// thousands would want a scan.)
 struct Plan {
   int32_t* table;
   const int32_t *kv_lens, *new_lens, *row_start, *free_pages;
@@ -391,7 +392,8 @@ void kv4_attention_f16(const Kv4Attention& a, hipStream_t s);
 
 // Which form, by the rows of one key / value head and the work there is (times in us; 32 query over 8 key / value heads of 128, bf16, unless it says otherwise):
 // * more than 64 rows: the form for chunks once its units of 128 rows fill the chip's 512 places (2048 tokens: 2 x 1024 queries 112 against 120 by
-//   tiles of 32, 64 sequences of 512 with 128 queries each 133 against 202; half as many units: 1 x 1024 queries 80 against 70).
+//   tiles of 32, 64 sequences of 512 with 128 queries each 133 against 202; half as many units: 1 x 1024 queries 80 against 70).  These are of 8 pairs of
+//   sequence and head or a multiple; other numbers leave XCDs idle in this form (kv4_attention_chunk_kernel), which the rule does not weigh.
 // * tiles of 32 once tiles of 16, four waves each, take more than half the places for waves (32 sequences of 2048, 20 rows: 27 against 29, 64 rows: 38 against
 //   49; fp32, 4 heads of 64, 32 rows, 256 units of 16: 12.7 against 8.6) -- but not for fp32 rows of more than 64, which spill (64 rows: 70 by tiles of
 //   16 against 76; 3 x 8 rows over 4 heads of 96, 128 sequences of 2000: 56 against 64).
@@ -419,6 +421,7 @@ Kv4Shape kv4_attention_shape(const Kv4Attention& a, Elem type) {
 // 44 / 29 / 22 / 26 / 34; 256 x 2048: 27 / 32).  Below 1024 tokens one (8 units x 600: 8.4 / 9.7).
 // Chunks: two ranges where units are few enough for long and short sequences to leave places empty at the end (4 sequences of 2500 to 8191 tokens,
 // 485 to 1000 queries: 529 against 617; all of 8192: 771 against 752; at 2048 tokens the join would cost a quarter: 260 against 207).
+// At most 32, so one sequence with few heads does not fill the chip (one token over 40000, 1 / 2 / 4 / 8 key / value heads: 15.7 / 15.7 / 15.6 / 16.6).
 int kv4_attention_splits(const Kv4Attention& a, Elem type) {
   const Kv4Shape shape = kv4_attention_shape(a, type);
   if (a.fixed || shape.kw != 4 || kv4_join_groups(a.rows, a.heads) > kGroupsMost) return 1;

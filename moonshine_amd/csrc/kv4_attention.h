@@ -13,8 +13,10 @@
 // No shared memory and no barrier in the walk; the next block's bytes are in flight while this one is computed.  (Batches of prompts have a form
 // of their own, below.)
 // 16 sequences of 12001 to 40000 tokens, 32 over 8 heads of 128, single bf16 tokens: 99 us and 5 for the join; the cache's 452 MB at 4.5 TB/s, HBM
-// bandwidth.  256 clips of 199 to 415 frames, 8 heads of 52, four fp32 beams each: 18.7 us for 43 MB, the vector unit -- three terms of q and p, and a wave's
-// beginning and end beside its six blocks.  One clip: 7.3 us, the latency of a launch, of the table, the bytes and 4 blocks a wave.
+// bandwidth.  256 clips of 199 to 415 frames, 8 heads of 52, four fp32 beams each: 18.8 us for 43 MB.  No unit is full (vector unit 39 % busy, the matrix unit's
+// 24 products a block come to a fifth of the time): it is a wave's chain of dependent products, three for each operand, the softmax between them, and its
+// beginning and end beside five or six blocks, in tiles of which 12 of 16 rows are empty.  One row a clip takes as long (18.4 us).  One clip: 7.2 us, the
+// latency of a launch, of the table, the bytes and 4 blocks a wave.
 //
 // Exactness: the cached values are exact in bf16.  q of fp16 / fp32 is the sum of 2 / 3 bf16 terms, p of 2 (3 for fp32 outputs) terms;
 // products, softmax statistics and sums are fp32.  The running maximum follows only when a score passes it by 2^8 (log2 units: 8), so
@@ -516,7 +518,8 @@ __global__ __launch_bounds__(256, (waves_wanted<M, E, RT>())) void kv4_attention
 // conflicts), two blocks deep: one barrier a block, the bytes of later blocks in flight meanwhile.
 // 4 sequences of 2500 to 8191 tokens with 485 to 1000 queries, 32 over 8 heads of 128, f16: 550 us and 36 for the join, 490 TFLOP/s of the formula's
 // products.  Two terms of q and of p make each of them two on the matrix unit, which is busy half of the time and the vector unit (softmax, terms, expanding)
-// the other half, at 2.1 GHz: what is left is their overlap.  Each wave expanding for itself: 740 us; operands read where they are used: 720.
+// the other half, at 2.1 GHz: what is left is their overlap.  Each wave expanding for itself: 740 us; operands read where they are used: 720.  bf16, one term
+// of q: 467 and 34 us; fp32, three of each: 861 and 34.
 // a wave's quarter of a block: keys' operands wave, wave + 4, ... of 2 M and values' groups (wave + 2) % 4, + 4, ... of M
 template <int M>
 struct QuarterKeys {
@@ -568,7 +571,8 @@ __global__ __attribute__((amdgpu_waves_per_eu((M <= 4 ? 2 : 1), (M <= 4 ? 2 : 1)
   const int quarter = lane >> 4, idx = lane & 15;
   const int heads_kv = a.cache.heads, per = a.heads / heads_kv;
   // workgroups go round the eight XCDs: pair p = (sequence, key / value head) belongs to XCD p % 8, so that the tiles that read one head's
-  // pages share an L2, and every XCD has heads of every sequence
+  // pages share an L2, and every XCD has heads of every sequence.  A number of pairs that is not a multiple of eight leaves XCDs idle: 1, 2, 3, 4 or 5 pairs
+  // take as long as 8 (2.3 ms, 4160 queries of 16 heads each over 8192 tokens of one head of 128, bf16), 9 as long as 16 (4.5 ms)
   const int turn = (int)blockIdx.x >> 3, unit = turn / a.nsplit, split = turn - unit * a.nsplit;
   const int group = unit / a.tiles, pair = group * 8 + ((int)blockIdx.x & 7), tile0 = unit - group * a.tiles;
   const int b = pair / heads_kv, head = pair - b * heads_kv, page_shift = a.cache.page_shift;
